@@ -47,6 +47,7 @@ enum {
 };
 
 enum { B200_F16 = 0, B200_BF16 = 1, B200_F32 = 2 };
+enum { B200_E4M3 = 3 }; /* 8-bit floating point with block scales: only where an entry point names it */
 
 /* Epilogue of the projection GEMM; replaces the Add / GELU / Add layers that follow MatMul in the unfused graph. */
 enum {
@@ -283,6 +284,120 @@ typedef struct B200LayerNormDesc {
     float        eps;
 } B200LayerNormDesc;
 B200_API int b200_add_layernorm_fwd(const B200LayerNormDesc* desc, b200_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------------------------
+ * 8-bit operands with block scales (no counterpart in the reference, whose 8-bit path is int8 for CNN layers).
+ * 128 consecutive values of a row share one fp32 scale.  With amax = max(largest magnitude of the block, 2^-40):
+ *   code = e4m3(v * (448 / amax)), scale = amax / 448, and the value stands for code * scale;
+ * quotient, product and scale are each rounded once to fp32, the code to nearest even.  A row's last block may be short.
+ * A block that holds an infinity or a NaN stands for no finite value (scale or codes are not finite).
+ * Activations: scale[b * ld_scale + row], b = column / 128 ("[ceil(K / 128), rows]", block-major: a warp's rows are contiguous).
+ * Weights [N, K]: one scale per 128 x 128 block, w_scale[(n / 128) * ceil(K / 128) + k / 128].
+ */
+
+/* Rows -> e4m3 + scales.  x: F16, BF16 or F32, row stride ldx; q: one byte per value, row stride ldq.
+ * Requirements: K % 16 == 0, rows of x and q on 16-byte boundaries (ldx * element size and ldq multiples of 16),
+ * ld_scale >= rows.  HBM-bound: reads x once, writes q and the scales. */
+typedef struct B200QuantizeFp8Desc {
+    const void* x;
+    void*       q;
+    float*      scale;
+    int64_t     rows, K;
+    int64_t     ldx, ldq, ld_scale;
+    int32_t     x_dtype;
+    int32_t     reserved_;
+} B200QuantizeFp8Desc;
+B200_API int b200_quantize_fp8(const B200QuantizeFp8Desc* desc, b200_stream_t stream);
+
+/* Weight pre-pack for b200_linear_fp8_fwd: fp32 w_kn[K, N] (TNN's MatMul layout) -> e4m3 w_nk[N, K] at row stride ld_dst
+ * and w_scale[ceil(N / 128), ceil(K / 128)].  K % 16 == 0, ld_dst % 16 == 0, w_nk 16-byte aligned. */
+B200_API int b200_pack_weight_fp8(const float* w_kn, int64_t K, int64_t N, int64_t ld_src, void* w_nk, int64_t ld_dst,
+                                  float* w_scale, b200_stream_t stream);
+
+/* (residual +) LayerNorm as b200_add_layernorm_fwd, whose result also (or, y = NULL, only) leaves as e4m3 + scales: the
+ * operand of the 8-bit GEMM behind it without another pass over the activation.  The codes are rounded from the fp32 result.
+ *   x, residual, y : dtype (F16 or BF16);  gamma, beta : fp32 [H];  q, scale : as b200_quantize_fp8.
+ *   Requirements: H % 16 == 0, H <= 4096, ldx, ldr, ldy % 8 == 0, ldq % 16 == 0, 16-byte aligned pointers. */
+typedef struct B200LayerNormFp8Desc {
+    const void*  x;
+    const void*  residual;
+    const float* gamma;
+    const float* beta;
+    void*        y;
+    void*        q;
+    float*       scale;
+    int64_t      rows, H;
+    int64_t      ldx, ldr, ldy, ldq, ld_scale;
+    int32_t      dtype;
+    float        eps;
+} B200LayerNormFp8Desc;
+B200_API int b200_add_layernorm_fp8_fwd(const B200LayerNormFp8Desc* desc, b200_stream_t stream);
+
+/* Projection / FFN GEMM on block-scaled e4m3 operands:
+ *   y[m, n] = epilogue(sum_b x_scale[b, m] * w_scale[n / 128, b] * sum_{k in block b} x[m, k] w_nk[n, k] + bias[n] (+ r[m, n]))
+ * with the epilogues of b200_linear_fwd.  Products and sums are fp32 (a block's sum in the tensor core, the sum over blocks
+ * in ascending order): a row's result depends on no other row, nor on M.
+ *   x [M, K], w_nk [N, K]: e4m3;  bias: fp32 [N] or NULL;  residual: res_dtype (F16 or BF16)
+ *   y: out_dtype F16, BF16, F32, or E4M3 with y_scale[ceil(N / 128), ld_y_scale] (the operand of a following 8-bit GEMM).
+ *   GELU and tanh use the fast forms of b200_linear_fwd (absolute deviation 3e-5, relative 2^-11) unless y is F32.
+ *   Requirements: K % 16 == 0, N % 8 == 0 (16 for E4M3), ldx, ldw % 16 == 0, ldy % 8 == 0 (16), ldr % 8 == 0, K <= 2^24,
+ *   ld_x_scale and ld_y_scale >= M, 16-byte aligned pointers (scales: 4-byte).
+ *   block_n: 0 = choose the tile; 128, 256: CTA-pair tiles (256 x block_n); -64 (not for E4M3), -128: single-CTA tiles. */
+typedef struct B200LinearFp8Desc {
+    const void*  x;
+    const void*  w_nk;
+    const float* x_scale;
+    const float* w_scale;
+    const float* bias;
+    const void*  residual;
+    void*        y;
+    float*       y_scale;
+    int64_t      M, N, K;
+    int64_t      ldx, ldw, ldr, ldy;
+    int64_t      ld_x_scale, ld_y_scale;
+    int32_t      out_dtype;
+    int32_t      res_dtype;
+    int32_t      epilogue;
+    int32_t      block_n;
+} B200LinearFp8Desc;
+B200_API int b200_linear_fp8_fwd(const B200LinearFp8Desc* desc, b200_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------------------------
+ * Sliding-window attention with first tokens that stay visible:
+ *   out[b, i, h] = softmax_j(scale * q[b, i, h] . k[b, j, h'] + mask_add[b, j]) . v[b, j, h'],   h' = h / (heads / kv_heads)
+ * over the keys j < kv_len[b] with j < sinks or pos - left <= j <= pos + right, where pos = q_start[b] + i is the position
+ * of query i.  (The reference has full attention only, as the chain that b200_attention_fwd replaces.)
+ *   left, right : window to either side of the query's position; negative = unlimited on that side; right = 0 is causal.
+ *   sinks       : how many first keys every query sees (0 = none).
+ *   kv_len      : int32 [B], keys of each sequence (clamped to Sk; <= 0: none), or NULL (= Sk).
+ *   q_start     : int32 [B], position of each sequence's first query, or NULL (= 0): Sq new tokens at the end of a cache
+ *                 of kv_len keys have q_start = kv_len - Sq.
+ *   mask_add    : fp32 [B, Sk] additive key mask or NULL.  A key whose value is <= mask_exclude_below (or NaN) is dropped.
+ *   A query that sees no key yields a row of zeros.  K and V rows that no query of the sequence may see (at or beyond kv_len,
+ *   or dropped by mask_add) may hold anything, infinities and NaN included.
+ *   q [B, Sq, ldq], k, v [B, Sk, ld*], out [B, Sq, ldo] : dtype (F16 / BF16), head h at columns h * 64; *_batch = elements
+ *   from one sequence to the next.  Requirements: head_dim == 64, kv_heads divides heads, all strides % 8 == 0, 16-byte
+ *   aligned pointers, Sq, Sk <= 2^24.
+ */
+typedef struct B200WindowAttentionDesc {
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    const float*   mask_add;
+    const int32_t* kv_len;
+    const int32_t* q_start;
+    void*          out;
+    int64_t        B, Sq, Sk;
+    int64_t        ldq, ldk, ldv, ldo;
+    int64_t        q_batch, k_batch, v_batch, o_batch;
+    int64_t        left, right, sinks;
+    int32_t        heads, kv_heads;
+    int32_t        head_dim;
+    int32_t        dtype;
+    float          scale;
+    float          mask_exclude_below;
+} B200WindowAttentionDesc;
+B200_API int b200_window_attention_fwd(const B200WindowAttentionDesc* desc, b200_stream_t stream);
 
 /* -------------------------------------------------------------------------------------------------------------------
  * One post-LN transformer-encoder layer (the fused form of the ~30 TNN layers of one BERT layer) and a whole encoder

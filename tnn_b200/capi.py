@@ -12,7 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TNN_B200_LIB", os.path.join(_HERE, "lib", "libtnn_b200.so"))
 
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3 = 0, 1, 2, 3
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL, EPI_BIAS_TANH = 0, 1, 2, 3
 
 OK = 0
@@ -64,6 +64,38 @@ class QAHeadDesc(_c.Structure):
                 ("N", _i32), ("x_dtype", _i32), ("out_n", _vp * 4)]
 
 
+class QuantizeFp8Desc(_c.Structure):
+    _fields_ = [("x", _vp), ("q", _vp), ("scale", _vp),
+                ("rows", _i64), ("K", _i64), ("ldx", _i64), ("ldq", _i64), ("ld_scale", _i64),
+                ("x_dtype", _i32), ("reserved_", _i32)]
+
+
+class LayerNormFp8Desc(_c.Structure):
+    _fields_ = [("x", _vp), ("residual", _vp), ("gamma", _vp), ("beta", _vp), ("y", _vp), ("q", _vp), ("scale", _vp),
+                ("rows", _i64), ("H", _i64),
+                ("ldx", _i64), ("ldr", _i64), ("ldy", _i64), ("ldq", _i64), ("ld_scale", _i64),
+                ("dtype", _i32), ("eps", _f32)]
+
+
+class LinearFp8Desc(_c.Structure):
+    _fields_ = [("x", _vp), ("w_nk", _vp), ("x_scale", _vp), ("w_scale", _vp), ("bias", _vp), ("residual", _vp),
+                ("y", _vp), ("y_scale", _vp),
+                ("M", _i64), ("N", _i64), ("K", _i64),
+                ("ldx", _i64), ("ldw", _i64), ("ldr", _i64), ("ldy", _i64),
+                ("ld_x_scale", _i64), ("ld_y_scale", _i64),
+                ("out_dtype", _i32), ("res_dtype", _i32), ("epilogue", _i32), ("block_n", _i32)]
+
+
+class WindowAttentionDesc(_c.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("mask_add", _vp), ("kv_len", _vp), ("q_start", _vp), ("out", _vp),
+                ("B", _i64), ("Sq", _i64), ("Sk", _i64),
+                ("ldq", _i64), ("ldk", _i64), ("ldv", _i64), ("ldo", _i64),
+                ("q_batch", _i64), ("k_batch", _i64), ("v_batch", _i64), ("o_batch", _i64),
+                ("left", _i64), ("right", _i64), ("sinks", _i64),
+                ("heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32),
+                ("scale", _f32), ("mask_exclude_below", _f32)]
+
+
 class EncoderLayerWeights(_c.Structure):
     _fields_ = [("w_qkv", _vp), ("b_qkv", _vp), ("w_o", _vp), ("b_o", _vp),
                 ("ln1_gamma", _vp), ("ln1_beta", _vp),
@@ -93,6 +125,11 @@ SYMBOLS = {
     "b200_embedding_layernorm_fwd": (_c.c_int, [_c.POINTER(EmbeddingDesc), _vp]),
     "b200_mask_from_input_mask": (_c.c_int, [_vp, _i64, _i64, _f32, _f32, _vp, _vp, _vp]),
     "b200_qa_head_fwd": (_c.c_int, [_c.POINTER(QAHeadDesc), _vp]),
+    "b200_quantize_fp8": (_c.c_int, [_c.POINTER(QuantizeFp8Desc), _vp]),
+    "b200_pack_weight_fp8": (_c.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "b200_add_layernorm_fp8_fwd": (_c.c_int, [_c.POINTER(LayerNormFp8Desc), _vp]),
+    "b200_linear_fp8_fwd": (_c.c_int, [_c.POINTER(LinearFp8Desc), _vp]),
+    "b200_window_attention_fwd": (_c.c_int, [_c.POINTER(WindowAttentionDesc), _vp]),
     "b200_encoder_workspace_bytes": (_c.c_size_t, [_i64, _i64, _i64, _c.c_int]),
     "b200_encoder_fwd": (_c.c_int, [_c.POINTER(EncoderDesc), _vp]),
     "b200_status_string": (_c.c_char_p, [_c.c_int]),

@@ -1,0 +1,528 @@
+// Projection / FFN GEMM on 8-bit operands with block scales:
+//   y[m, n] = epilogue(sum_b xs[b, m] * ws[n / 128, b] * sum_{k in block b} x8[m, k] w8[n, k] + bias[n] (+ r[m, n])).
+//
+// The scales change every 128 values of K, so the tensor cores may not add across blocks.  A k-block of a pipeline stage is
+// exactly one scale block (128 e4m3 values = one 128-byte swizzled row): its four UMMAs (kind::f8f6f4, K = 32 each) start a
+// fresh accumulator in one of NBUF TMEM buffers, and the epilogue warps add scale * buffer to fp32 sums that stay in their
+// registers for the whole tile (thread = row, COLS columns), while the tensor pipe fills the other buffers.  Products are
+// exact in fp32; the sum inside a block is the tensor core's fp32 accumulation, the sum over blocks one fp32 FMA each, in
+// ascending order whatever the tile, so a row's result depends on neither the batch nor the tile chosen.
+//
+// CG = 2: pairs of SMs (cta_group::2) on a 256 x BN tile, each CTA loading its 128 rows of x and BN / 2 rows of w;
+// CG = 1: one SM on 128 x BN, for launches of few rows.  Roles as in linear_pair.cu: warp 0 TMA producer, warp 1 TMEM
+// allocation and UMMA issue (in the leader CTA), the other EW warps scale, add and store.
+#include "fp8.cuh"
+#include "pair.cuh"
+
+namespace b200 {
+namespace lin {
+
+namespace {
+
+enum { kOutHalf = 0, kOutF32 = 1, kOutF8 = 2 };
+
+struct LinearFp8Params {
+    const float* x_scale;
+    const float* w_scale;
+    const float* bias;
+    const void* residual;
+    float* y_scale;
+    int M, N;
+    int num_n_tiles, num_tiles, num_k_blocks, w_blocks;   // w_blocks = ceil(N / 128)
+    int x_rows;                                           // rows of x in a load box
+    int out_dtype, res_dtype, epilogue;
+    long long ld_xs, ld_ys, ldr;
+    uint32_t idesc;
+    unsigned int* status;
+};
+
+template <int CG, int BN, int EW>
+struct Fp8Cfg {
+    static constexpr int THREADS = 64 + 32 * EW;
+    static constexpr int COLS = BN / (EW / 4);           // accumulator columns per epilogue warp
+    static constexpr int NBUF = BN == 256 ? 2 : 4;       // TMEM buffers of BN columns
+    static constexpr int TMEM_COLS = BN * NBUF;
+    static constexpr int A_BYTES = 128 * 128;
+    static constexpr int B_BYTES = BN / CG * 128;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STRIP_BYTES = 32 * 128;         // one warp's output staging: 32 rows of 128 bytes
+    static constexpr int TAIL_BYTES = EW * STRIP_BYTES + 512;
+    static constexpr int FIT = (227 * 1024 - 1024 - TAIL_BYTES) / STAGE_BYTES;
+    static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int OUT_OFFSET = STAGES * STAGE_BYTES;
+    static constexpr int BAR_OFFSET = OUT_OFFSET + EW * STRIP_BYTES;
+    static constexpr int SMEM_BYTES = OUT_OFFSET + TAIL_BYTES + 1024;
+    static_assert(STAGES >= 3 && TMEM_COLS <= 512 && COLS % 32 == 0, "tile does not fit");
+};
+
+template <int CG, int BN, int EW, int OUT>
+__global__ void __launch_bounds__(64 + 32 * EW, 1)
+linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_y, const LinearFp8Params p) {
+    using C = Fp8Cfg<CG, BN, EW>;
+    constexpr int STAGES = C::STAGES, NBUF = C::NBUF, COLS = C::COLS;
+    extern __shared__ uint8_t smem_raw[];
+    // Rounding up gives the same offset in both CTAs of a pair: the dynamic window starts at the same place in each.
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFFSET);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + NBUF;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + NBUF);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+    const bool leader = rank == 0;
+    const int group = blockIdx.x / CG;
+    const int num_groups = gridDim.x / CG;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);    // the leader's expect_tx arrival
+            mbar_init(&empty[s], 1);   // one commit per use
+        }
+        for (int b = 0; b < NBUF; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], CG * EW);   // leader's copy: epilogue warps of all its CTAs
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        prefetch_tmap(&tm_x);
+        prefetch_tmap(&tm_w);
+    }
+    if (warp == 1) {
+        if (CG == 2) {
+            tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, C::TMEM_COLS);
+            tmem_relinquish();
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();   // the peer's barriers and TMEM are set up before anything is signalled
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        // The weights' way from HBM to L2 starts while the previous kernel of the stream drains (a hint, no data is taken).
+        const int row_boxes = (p.N + BN / CG - 1) / (BN / CG);
+        for (int b = blockIdx.x; b < p.num_k_blocks * row_boxes; b += gridDim.x)
+            tma_prefetch_l2_2d(&tm_w, (b % p.num_k_blocks) * 64, (b / p.num_k_blocks) * (BN / CG));
+    }
+    pdl_wait();
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer (every CTA its own part)
+        if (elect_one()) {
+            uint32_t st = 0, ph = 0;
+            bool ok = true;
+            const uint32_t bytes = CG * (static_cast<uint32_t>(p.x_rows) * 128 + C::B_BYTES);
+            for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
+                const int x_row = tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128;
+                const int w_row = tile % p.num_n_tiles * BN + static_cast<int>(rank) * (BN / CG);
+                for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+                    if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    uint8_t* a = smem + st * C::STAGE_BYTES;
+                    uint8_t* b = a + C::A_BYTES;
+                    if (leader) mbar_expect_tx(&full[st], bytes);
+                    // the maps count 16-bit units: a k-block is 64 of them
+                    if (CG == 2) {
+                        const uint32_t bar = leader_addr(&full[st]);
+                        tma_load_2d_pair(a, &tm_x, bar, kb * 64, x_row);
+                        tma_load_2d_pair(b, &tm_w, bar, kb * 64, w_row);
+                    } else {
+                        tma_load_2d(a, &tm_x, &full[st], kb * 64, x_row);
+                        tma_load_2d(b, &tm_w, &full[st], kb * 64, w_row);
+                    }
+                    if (++st == STAGES) { st = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok) {
+                for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ UMMA issuer (leader CTA only)
+        if (leader && elect_one()) {
+            uint32_t st = 0, ph = 0, buf = 0, bph = 0;
+            bool ok = true;
+            const uint64_t a_desc0 = make_smem_desc_sw128(smem_u32(smem));
+            const uint64_t b_desc0 = make_smem_desc_sw128(smem_u32(smem + C::A_BYTES));
+            for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
+                for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+                    if (!mbar_wait(&acc_empty[buf], bph ^ 1u, abort_flag) || !mbar_wait(&full[st], ph, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const uint32_t d_tmem = tmem_base + buf * BN;
+                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
+                    const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (CG == 2) umma_f8_ss_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, p.idesc, k != 0 ? 1u : 0u);
+                        else umma_f8_ss(d_tmem, a_desc + 2 * k, b_desc + 2 * k, p.idesc, k != 0 ? 1u : 0u);
+                    }
+                    umma_f8_commit(&empty[st], CG == 2);
+                    umma_f8_commit(&acc_full[buf], CG == 2);
+                    if (++st == STAGES) { st = 0; ph ^= 1u; }
+                    if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ scale, add, store (own 128 rows)
+        const int ew = warp - 2;
+        const int quarter = warp & 3;
+        const int col_first = (ew >> 2) * COLS;
+        uint8_t* strip = smem + C::OUT_OFFSET + ew * C::STRIP_BYTES;
+        uint8_t* srow = strip + lane * 128;
+        const int sw = lane & 7;            // 128-byte swizzle: 16-byte piece i of row r lies at i ^ (r & 7)
+        const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_first;
+        uint32_t buf = 0, bph = 0;
+        bool ok = true;
+        for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
+            const int row0 = tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128 + quarter * 32;
+            const int row = row0 + lane;
+            const int n_first = tile % p.num_n_tiles * BN + col_first;
+            const bool row_ok = row < p.M;
+            // the scale of this thread's row and of the warp's columns, one k-block ahead
+            const float* xs = p.x_scale + (row_ok ? row : 0);
+            const int wb = n_first / fp8::kBlock;
+            const float* ws = p.w_scale + static_cast<long long>(wb < p.w_blocks ? wb : p.w_blocks - 1) * p.num_k_blocks;
+            float s_next = __ldg(xs) * __ldg(ws);
+            uint64_t acc[COLS / 2];
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
+            for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+                const uint64_t s2 = pack_f32x2(s_next, s_next);
+                if (kb + 1 < p.num_k_blocks) s_next = __ldg(xs + (kb + 1) * p.ld_xs) * __ldg(ws + kb + 1);
+                if (!mbar_wait(&acc_full[buf], bph, abort_flag)) { ok = false; break; }
+                __syncwarp();
+                tcgen05_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(tacc + buf * BN + c * 32, r);
+                    tmem_ld_wait(r);
+                    if (c == COLS / 32 - 1) {   // the buffer is in registers: hand it back
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (CG == 2 && !leader) mbar_arrive_leader(&acc_empty[buf]);
+                            else mbar_arrive(&acc_empty[buf]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        acc[c * 16 + j] = fma_f32x2(pack_f32x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2,
+                                                    acc[c * 16 + j]);
+                }
+                if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+            }
+            if (!ok) break;
+
+            // bias, activation, residual
+            uint32_t bits = 0;
+#pragma unroll
+            for (int c = 0; c < COLS / 32; ++c) {
+                const int n0 = n_first + c * 32;
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1]);
+                if (p.bias != nullptr) {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+                        if (n0 + g * 4 < p.N) {
+                            const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0) + g);
+                            v[g * 4 + 0] += b.x;
+                            v[g * 4 + 1] += b.y;
+                            v[g * 4 + 2] += b.z;
+                            v[g * 4 + 3] += b.w;
+                        }
+                }
+                if (p.epilogue == B200_EPI_BIAS_GELU) {
+                    if (OUT == kOutF32) {   // nothing rounds the result: the library's erf
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678118654752f));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) gelu_erf_x2(v[j], v[j + 1]);
+                    }
+                } else if (p.epilogue == B200_EPI_BIAS_TANH) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (OUT == kOutF32) v[j] = tanhf(v[j]);
+                        else asm("tanh.approx.f32 %0, %1;" : "=f"(v[j]) : "f"(v[j]));
+                    }
+                } else if (p.epilogue == B200_EPI_BIAS_RESIDUAL && row_ok) {
+                    const uint16_t* rp = static_cast<const uint16_t*>(p.residual) + row * p.ldr + n0;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        if (n0 + g * 8 < p.N) {
+                            const uint4 q = __ldg(reinterpret_cast<const uint4*>(rp + g * 8));
+                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = unpack2(w[e], p.res_dtype);
+                                v[g * 8 + 2 * e] += f.x;
+                                v[g * 8 + 2 * e + 1] += f.y;
+                            }
+                        }
+                }
+                if (OUT == kOutF8) {
+                    // columns at or beyond N are zeros (no weight, no bias, no residual): they do not move the maximum
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) bits = max(bits, fp8::abs_bits(v[j]));
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[c * 16 + j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
+                    continue;
+                }
+                constexpr int PER_STRIP = OUT == kOutF32 ? 1 : 2;   // 32-column chunks in a strip
+                if (c % PER_STRIP == 0) {
+                    if (lane == 0) tma_store_wait_read<0>();   // the strip's previous store has read it
+                    __syncwarp();
+                }
+                if (OUT == kOutF32) {
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+                        *reinterpret_cast<float4*>(srow + ((g ^ sw) << 4)) =
+                            make_float4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint4 q;
+                        q.x = pack2(v[g * 8 + 0], v[g * 8 + 1], p.out_dtype);
+                        q.y = pack2(v[g * 8 + 2], v[g * 8 + 3], p.out_dtype);
+                        q.z = pack2(v[g * 8 + 4], v[g * 8 + 5], p.out_dtype);
+                        q.w = pack2(v[g * 8 + 6], v[g * 8 + 7], p.out_dtype);
+                        *reinterpret_cast<uint4*>(srow + ((((c & 1) * 4 + g) ^ sw) << 4)) = q;
+                    }
+                }
+                if (c % PER_STRIP == PER_STRIP - 1) {
+                    fence_async_proxy_shared();
+                    __syncwarp();
+                    const int n_strip = n_first + (c / PER_STRIP) * PER_STRIP * 32;
+                    if (lane == 0 && n_strip < p.N && row0 < p.M) {   // the store clips rows and columns outside y
+                        tma_store_2d(&tm_y, strip, OUT == kOutF32 ? 2 * n_strip : n_strip, row0);
+                        tma_store_commit();
+                    }
+                }
+            }
+            if (OUT == kOutF8) {
+                const float amax = fp8::amax_of_bits(bits);
+                const float enc = fp8::encode_scale(amax);
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int g = 0; g < COLS / 16; ++g) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float a0, a1, a2, a3;
+                        unpack_f32x2(acc[g * 8 + e * 2], a0, a1);
+                        unpack_f32x2(acc[g * 8 + e * 2 + 1], a2, a3);
+                        w[e] = fp8::pack4(a0 * enc, a1 * enc, a2 * enc, a3 * enc);
+                    }
+                    *reinterpret_cast<uint4*>(srow + ((g ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (row_ok && n_first < p.N) p.y_scale[wb * p.ld_ys + row] = fp8::decode_scale(amax);
+                fence_async_proxy_shared();
+                __syncwarp();
+                if (lane == 0 && n_first < p.N && row0 < p.M) {
+                    tma_store_2d(&tm_y, strip, n_first / 2, row0);
+                    tma_store_commit();
+                }
+            }
+        }
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+    }
+
+    // ---------------------------------------------------------------- teardown
+    tcgen05_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();   // neither CTA frees TMEM or leaves while the other may still signal or read it
+    if (warp == 1) {
+        tcgen05_fence_after();
+        if (CG == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+        else tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) atomicOr(p.status, 1u);
+}
+
+// Launch with a cluster dimension (CG = 2) beside the programmatic-serialization attribute.
+template <int CG, typename... KArgs, typename... Args>
+cudaError_t launch_groups(void (*kernel)(KArgs...), unsigned ctas, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (CG == 2) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = 2;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = static_cast<unsigned>(n);
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// CTA groups that can be resident at once (a persistent grid must not exceed it), looked up once per device and instance.
+template <int CG, int BN, int EW, int OUT>
+int resident_groups(int sms) {
+    using C = Fp8Cfg<CG, BN, EW>;
+    static PerDeviceOnce once;
+    static int groups[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const bool ready = once.ensure(dev, [&]() {
+        if (cudaFuncSetAttribute(linear_fp8_kernel<CG, BN, EW, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
+            cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        int n = sms;
+        if (CG == 2) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+            cfg.blockDim = dim3(C::THREADS);
+            cfg.dynamicSmemBytes = C::SMEM_BYTES;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 2;
+            attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, linear_fp8_kernel<CG, BN, EW, OUT>, &cfg) != cudaSuccess || n <= 0) {
+                cudaGetLastError();
+                n = sms / 2;
+            }
+            if (n > sms / 2) n = sms / 2;
+        }
+        groups[dev] = n;
+        return true;
+    });
+    return ready ? groups[dev] : 0;
+}
+
+template <int CG, int BN, int EW, int OUT>
+int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) {
+    using C = Fp8Cfg<CG, BN, EW>;
+    const int groups = resident_groups<CG, BN, EW, OUT>(sms);
+    if (groups <= 0) return B200_ERR_LAUNCH;
+    // Rows that do not exist are not fetched where all rows fit one box: what the stage holds there feeds no stored row.
+    const int x_rows = CG == 1 && d.M < 128 ? static_cast<int>((d.M + 7) / 8 * 8) : 128;
+    CUtensorMap tx, tw, ty;
+    {   // two e4m3 values as one 16-bit element
+        const uint64_t xd[2] = {static_cast<uint64_t>(d.K / 2), static_cast<uint64_t>(d.M)};
+        const uint64_t xs[1] = {static_cast<uint64_t>(d.ldx)};
+        const uint32_t xb[2] = {64, static_cast<uint32_t>(x_rows)};
+        const uint64_t wd[2] = {static_cast<uint64_t>(d.K / 2), static_cast<uint64_t>(d.N)};
+        const uint64_t ws[1] = {static_cast<uint64_t>(d.ldw)};
+        const uint32_t wb[2] = {64, BN / CG};
+        const uint64_t cols = OUT == kOutF32 ? 2 * static_cast<uint64_t>(d.N) : (OUT == kOutF8 ? d.N / 2 : d.N);
+        const uint64_t yd[2] = {cols, static_cast<uint64_t>(d.M)};
+        const uint64_t ys[1] = {static_cast<uint64_t>(d.ldy) * (OUT == kOutF32 ? 4 : (OUT == kOutF8 ? 1 : 2))};
+        const uint32_t yb[2] = {64, 32};
+        if (!get_tensor_map(&tx, d.x, 2, xd, xs, xb) || !get_tensor_map(&tw, d.w_nk, 2, wd, ws, wb) ||
+            !get_tensor_map(&ty, d.y, 2, yd, ys, yb))
+            return B200_ERR_DRIVER;
+    }
+    LinearFp8Params p;
+    p.x_scale = d.x_scale;
+    p.w_scale = d.w_scale;
+    p.bias = d.bias;
+    p.residual = d.residual;
+    p.y_scale = d.y_scale;
+    p.M = static_cast<int>(d.M);
+    p.N = static_cast<int>(d.N);
+    p.num_n_tiles = (p.N + BN - 1) / BN;
+    const long long tiles = (d.M + 128 * CG - 1) / (128 * CG) * p.num_n_tiles;
+    if (tiles > 0x7fffffffll) return B200_ERR_UNSUPPORTED;
+    p.num_tiles = static_cast<int>(tiles);
+    p.num_k_blocks = static_cast<int>((d.K + 127) / 128);
+    p.w_blocks = (p.N + 127) / 128;
+    p.x_rows = x_rows;
+    p.out_dtype = d.out_dtype;
+    p.res_dtype = d.res_dtype;
+    p.epilogue = d.epilogue;
+    p.ld_xs = d.ld_x_scale;
+    p.ld_ys = d.ld_y_scale;
+    p.ldr = d.ldr;
+    p.idesc = make_idesc_f16(128 * CG, BN, 0, 0, 0);   // format code 0 of kind::f8f6f4 = e4m3
+    p.status = device_status_ptr();
+    const int used = p.num_tiles < groups ? p.num_tiles : groups;
+    launch_groups<CG>(linear_fp8_kernel<CG, BN, EW, OUT>, static_cast<unsigned>(used * CG), C::THREADS, C::SMEM_BYTES, stream, tx, tw,
+                      ty, p);
+    count_launch();
+    return check_launch();
+}
+
+template <int CG, int BN>
+int launch_by_output(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) {
+    // e4m3 output: a thread holds a whole scale block of its row, 128 columns
+    constexpr int EW = BN == 64 ? 4 : 8, EW8 = BN == 256 ? 8 : 4;
+    if (d.out_dtype == B200_E4M3) {
+        if constexpr (BN >= 128) return launch_linear_fp8<CG, BN, EW8, kOutF8>(d, stream, sms);
+        else return B200_ERR_PARAM;
+    }
+    if (d.out_dtype == B200_F32) return launch_linear_fp8<CG, BN, EW, kOutF32>(d, stream, sms);
+    return launch_linear_fp8<CG, BN, EW, kOutHalf>(d, stream, sms);
+}
+
+int validate_linear_fp8(const B200LinearFp8Desc* d) {
+    if (!d || !d->x || !d->w_nk || !d->y || !d->x_scale || !d->w_scale) return B200_ERR_PARAM;
+    if (d->M < 0 || d->N <= 0 || d->K <= 0) return B200_ERR_PARAM;
+    if (d->M > (1ll << 30) || d->N > (1ll << 30) || d->K > (1ll << 24)) return B200_ERR_UNSUPPORTED;
+    const bool f8 = d->out_dtype == B200_E4M3;
+    if (!f8 && !is_half_dtype(d->out_dtype) && d->out_dtype != B200_F32) return B200_ERR_PARAM;
+    if (d->epilogue < B200_EPI_BIAS || d->epilogue > B200_EPI_BIAS_TANH) return B200_ERR_PARAM;
+    const int64_t per = f8 ? 16 : 8;
+    if ((d->K % 16) || (d->N % per) || (d->ldx % 16) || (d->ldw % 16) || (d->ldy % per)) return B200_ERR_PARAM;
+    if (d->ldx < d->K || d->ldw < d->K || d->ldy < d->N || d->ld_x_scale < d->M) return B200_ERR_PARAM;
+    if (f8 && (!d->y_scale || d->ld_y_scale < d->M)) return B200_ERR_PARAM;
+    if (!aligned16(d->x) || !aligned16(d->w_nk) || !aligned16(d->y) || (d->bias && !aligned16(d->bias))) return B200_ERR_PARAM;
+    if (d->epilogue == B200_EPI_BIAS_RESIDUAL &&
+        (!d->residual || !is_half_dtype(d->res_dtype) || (d->ldr % 8) || d->ldr < d->N || !aligned16(d->residual)))
+        return B200_ERR_PARAM;
+    if (d->block_n != 0 && d->block_n != 128 && d->block_n != 256 && d->block_n != -128 && (d->block_n != -64 || f8)) return B200_ERR_PARAM;
+    return B200_OK;
+}
+
+}  // namespace
+}  // namespace lin
+}  // namespace b200
+
+extern "C" int b200_linear_fp8_fwd(const B200LinearFp8Desc* d, b200_stream_t stream_) {
+    using namespace b200;
+    using namespace b200::lin;
+    const int valid = validate_linear_fp8(d);
+    if (valid != B200_OK || d->M == 0) return valid;
+    const int sms = device_sm_count();
+    if (sms <= 0) return B200_ERR_NOT_SM100;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    int bn = d->block_n;
+    if (bn == 0) bn = d->M <= 128 ? (d->out_dtype == B200_E4M3 ? -128 : -64) : 256;
+    switch (bn) {
+        case 256: return launch_by_output<2, 256>(*d, stream, sms);
+        case 128: return launch_by_output<2, 128>(*d, stream, sms);
+        case -128: return launch_by_output<1, 128>(*d, stream, sms);
+        default: return launch_by_output<1, 64>(*d, stream, sms);
+    }
+}

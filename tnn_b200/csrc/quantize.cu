@@ -1,0 +1,329 @@
+// What makes the 8-bit operands of linear_fp8.cu: the row quantizer, (residual +) LayerNorm with an 8-bit result, and the
+// one-time weight pre-pack.  All HBM-bound: every input is read once, every output written once.
+#include "fp8.cuh"
+#include "linear_common.cuh"
+
+namespace b200 {
+namespace {
+
+// ---------------------------------------------------------------- rows -> e4m3 + scales
+// A group of 8 lanes owns one block of 128 values, 16 per lane: 16-byte loads and one 16-byte store per lane, the block's
+// largest magnitude by three shuffles.  A warp holds four blocks, UNROLL of them per lane in flight.
+template <int DT>
+struct Raw16 {   // 16 consecutive elements as loaded
+    static constexpr int Q = DT == B200_F32 ? 4 : 2;
+    uint4 q[Q];
+};
+template <int DT>
+__device__ __forceinline__ void decode16(const Raw16<DT>& r, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < Raw16<DT>::Q; ++i) {
+        const uint32_t w[4] = {r.q[i].x, r.q[i].y, r.q[i].z, r.q[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (DT == B200_F32) {
+                v[i * 4 + e] = __uint_as_float(w[e]);
+            } else {
+                const float2 f = unpack2(w[e], DT);
+                v[i * 8 + e * 2] = f.x;
+                v[i * 8 + e * 2 + 1] = f.y;
+            }
+        }
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) quantize_fp8_kernel(B200QuantizeFp8Desc d, long long items, int blocks) {
+    constexpr int UNROLL = DT == B200_F32 ? 2 : 4;
+    constexpr int kGroups = 32;   // blocks of 128 values per CTA and step
+    pdl_launch_dependents();
+    pdl_wait();
+    const int group = threadIdx.x >> 3, sub = threadIdx.x & 7;
+    const long long step = static_cast<long long>(gridDim.x) * kGroups;
+    for (long long i0 = static_cast<long long>(blockIdx.x) * kGroups + group; i0 - group < items; i0 += step * UNROLL) {
+        Raw16<DT> raw[UNROLL];
+        bool in[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const long long i = i0 + u * step;
+            const long long row = i / blocks;
+            const long long col = (i - row * blocks) * fp8::kBlock + sub * 16;
+            in[u] = i < items && col < d.K;
+#pragma unroll
+            for (int k = 0; k < Raw16<DT>::Q; ++k) raw[u].q[k] = make_uint4(0, 0, 0, 0);
+            if (in[u]) {
+                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(d.x) +
+                                                                (row * d.ldx + col) * (DT == B200_F32 ? 4 : 2));
+#pragma unroll
+                for (int k = 0; k < Raw16<DT>::Q; ++k) raw[u].q[k] = __ldg(p + k);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const long long i = i0 + u * step;
+            const long long row = i / blocks;
+            const int kb = static_cast<int>(i - row * blocks);
+            float v[16];
+            decode16<DT>(raw[u], v);
+            uint32_t bits = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bits = max(bits, fp8::abs_bits(v[e]));
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+            const float amax = fp8::amax_of_bits(bits);
+            const float enc = fp8::encode_scale(amax);
+            if (in[u]) {
+                uint4 q;
+                q.x = fp8::pack4(v[0] * enc, v[1] * enc, v[2] * enc, v[3] * enc);
+                q.y = fp8::pack4(v[4] * enc, v[5] * enc, v[6] * enc, v[7] * enc);
+                q.z = fp8::pack4(v[8] * enc, v[9] * enc, v[10] * enc, v[11] * enc);
+                q.w = fp8::pack4(v[12] * enc, v[13] * enc, v[14] * enc, v[15] * enc);
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(d.q) + row * d.ldq + kb * fp8::kBlock + sub * 16) = q;
+                if (sub == 0) d.scale[kb * d.ld_scale + row] = fp8::decode_scale(amax);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- (residual +) LayerNorm -> half and e4m3 + scales
+// A warp per row; a lane holds NV groups of 8 consecutive elements (group g of the lane = elements (g * 32 + lane) * 8 ..),
+// so that 16 lanes hold a block of 128 and its largest magnitude is four shuffles away.  The 8-bit result is rounded from
+// the 32-bit one, not from its half-precision copy.  gamma and beta in shared memory, the next row's loads in flight while
+// this one is reduced.
+__device__ __forceinline__ void decode8(const uint4& q, int dtype, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2(w[e], dtype);
+        v[2 * e] = f.x;
+        v[2 * e + 1] = f.y;
+    }
+}
+
+template <int NV, int DT, bool RESID>
+__global__ void __launch_bounds__(256) add_layernorm_fp8_kernel(B200LayerNormFp8Desc d) {
+    extern __shared__ float gb[];   // gamma, then beta: group-major, the 8 elements of a lane's group in two float4 planes
+    const int lane = threadIdx.x & 31;
+    const int H = static_cast<int>(d.H);
+    const int groups = H >> 3;
+    float* beta_s = gb + NV * 256;
+    pdl_launch_dependents();
+    pdl_wait();   // gamma and beta too may have been written by the kernel in front
+    const long long nwarps = static_cast<long long>(gridDim.x) * 8;
+    uint4 raw[NV], res[RESID ? NV : 1];
+    auto fetch = [&](long long row) {
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+            const int gi = g * 32 + lane;
+            raw[g] = make_uint4(0, 0, 0, 0);
+            if (RESID) res[g] = make_uint4(0, 0, 0, 0);
+            if (gi < groups) {
+                raw[g] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(d.x) + row * d.ldx + gi * 8));
+                if (RESID) res[g] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(d.residual) + row * d.ldr + gi * 8));
+            }
+        }
+    };
+    long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (row < d.rows) fetch(row);
+    for (int i = threadIdx.x; i < NV * 256; i += 256) {
+        const int g = i >> 8, r = i & 255, l = r >> 3, e = r & 7;
+        const int at = (g * 2 + (e >> 2)) * 128 + l * 4 + (e & 3);   // conflict-free float4 per lane
+        gb[at] = i < H ? __ldg(d.gamma + i) : 0.f;
+        beta_s[at] = i < H ? __ldg(d.beta + i) : 0.f;
+    }
+    __syncthreads();
+    const float inv_h = 1.0f / static_cast<float>(H);
+    for (; row < d.rows; row += nwarps) {
+        float v[NV][8];
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+            decode8(raw[g], DT, v[g]);
+            if (RESID) {
+                float r[8];
+                decode8(res[g], DT, r);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[g][e] += r[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += v[g][e];
+        }
+        if (row + nwarps < d.rows) fetch(row + nwarps);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float mean = sum * inv_h;
+        float sq = 0.f;
+#pragma unroll
+        for (int g = 0; g < NV; ++g)
+            if (g * 32 + lane < groups) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[g][e] -= mean;
+                    sq = fmaf(v[g][e], v[g][e], sq);
+                }
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        const float rstd = 1.0f / sqrtf(fmaf(sq, inv_h, d.eps));
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+            const int gi = g * 32 + lane;
+            uint32_t bits = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 gm = *reinterpret_cast<const float4*>(gb + (g * 2 + h) * 128 + lane * 4);
+                const float4 bt = *reinterpret_cast<const float4*>(beta_s + (g * 2 + h) * 128 + lane * 4);
+                v[g][h * 4 + 0] = fmaf(v[g][h * 4 + 0] * rstd, gm.x, bt.x);
+                v[g][h * 4 + 1] = fmaf(v[g][h * 4 + 1] * rstd, gm.y, bt.y);
+                v[g][h * 4 + 2] = fmaf(v[g][h * 4 + 2] * rstd, gm.z, bt.z);
+                v[g][h * 4 + 3] = fmaf(v[g][h * 4 + 3] * rstd, gm.w, bt.w);
+            }
+            if (gi < groups) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bits = max(bits, fp8::abs_bits(v[g][e]));
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+            if (gi < groups) {
+                const float amax = fp8::amax_of_bits(bits);
+                const float enc = fp8::encode_scale(amax);
+                if (d.y) {
+                    uint4 q;
+                    q.x = pack2t<DT>(v[g][0], v[g][1]);
+                    q.y = pack2t<DT>(v[g][2], v[g][3]);
+                    q.z = pack2t<DT>(v[g][4], v[g][5]);
+                    q.w = pack2t<DT>(v[g][6], v[g][7]);
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(d.y) + row * d.ldy + gi * 8) = q;
+                }
+                uint2 c;
+                c.x = fp8::pack4(v[g][0] * enc, v[g][1] * enc, v[g][2] * enc, v[g][3] * enc);
+                c.y = fp8::pack4(v[g][4] * enc, v[g][5] * enc, v[g][6] * enc, v[g][7] * enc);
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(d.q) + row * d.ldq + gi * 8) = c;
+                if ((lane & 15) == 0) d.scale[(gi >> 4) * d.ld_scale + row] = fp8::decode_scale(amax);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- weight pre-pack
+// fp32 w_kn[K, N] -> e4m3 w_nk[N, K] and one scale per 128 x 128 block.  A CTA per block; runs once, at load time: the
+// block is read twice (its largest magnitude first), transposed through shared memory 32 columns of N at a time.
+__global__ void __launch_bounds__(256) pack_weight_fp8_kernel(const float* src, long long K, long long N, long long ld_src,
+                                                              uint8_t* dst, long long ld_dst, float* scale, int kblocks) {
+    __shared__ uint32_t red[8];
+    __shared__ float tile[128][33];
+    const long long k0 = static_cast<long long>(blockIdx.x) * 128, n0 = static_cast<long long>(blockIdx.y) * 128;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    uint32_t bits = 0;
+    for (int k = ty; k < 128 && k0 + k < K; k += 8)
+        for (int n = tx; n < 128 && n0 + n < N; n += 32) bits = max(bits, fp8::abs_bits(src[(k0 + k) * ld_src + n0 + n]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    if (tx == 0) red[ty] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) bits = max(bits, red[w]);
+    const float amax = fp8::amax_of_bits(bits);
+    const float enc = fp8::encode_scale(amax);
+    if (threadIdx.x == 0) scale[static_cast<long long>(blockIdx.y) * kblocks + blockIdx.x] = fp8::decode_scale(amax);
+    for (int c = 0; c < 128; c += 32) {
+        __syncthreads();
+        for (int k = ty; k < 128; k += 8)
+            tile[k][tx] = (k0 + k < K && n0 + c + tx < N) ? src[(k0 + k) * ld_src + n0 + c + tx] : 0.f;
+        __syncthreads();
+        for (int n = ty; n < 32 && n0 + c + n < N; n += 8)
+            if (k0 + tx * 4 < K)   // K is a multiple of 16
+                *reinterpret_cast<uint32_t*>(dst + (n0 + c + n) * ld_dst + k0 + tx * 4) =
+                    fp8::pack4(tile[tx * 4][n] * enc, tile[tx * 4 + 1][n] * enc, tile[tx * 4 + 2][n] * enc, tile[tx * 4 + 3][n] * enc);
+    }
+}
+
+template <int NV, int DT>
+void launch_layernorm_fp8(unsigned grid, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
+    const size_t smem = static_cast<size_t>(NV) * 256 * 2 * sizeof(float);
+    if (d.residual) launch_kernel(add_layernorm_fp8_kernel<NV, DT, true>, dim3(grid), dim3(256), smem, stream, d);
+    else launch_kernel(add_layernorm_fp8_kernel<NV, DT, false>, dim3(grid), dim3(256), smem, stream, d);
+}
+
+template <int DT>
+void choose_layernorm_fp8(int nv, unsigned grid, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
+    if (nv <= 1) launch_layernorm_fp8<1, DT>(grid, stream, d);
+    else if (nv <= 2) launch_layernorm_fp8<2, DT>(grid, stream, d);
+    else if (nv <= 3) launch_layernorm_fp8<3, DT>(grid, stream, d);
+    else if (nv <= 4) launch_layernorm_fp8<4, DT>(grid, stream, d);
+    else if (nv <= 8) launch_layernorm_fp8<8, DT>(grid, stream, d);
+    else launch_layernorm_fp8<16, DT>(grid, stream, d);
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" {
+
+int b200_quantize_fp8(const B200QuantizeFp8Desc* d, b200_stream_t stream_) {
+    using namespace b200;
+    if (!d || !d->x || !d->q || !d->scale) return B200_ERR_PARAM;
+    if (d->rows < 0 || d->K <= 0) return B200_ERR_PARAM;
+    if (d->x_dtype != B200_F16 && d->x_dtype != B200_BF16 && d->x_dtype != B200_F32) return B200_ERR_PARAM;
+    const int64_t per16 = d->x_dtype == B200_F32 ? 4 : 8;   // elements in 16 bytes
+    if ((d->K % 16) || (d->ldx % per16) || (d->ldq % 16) || d->ldx < d->K || d->ldq < d->K || d->ld_scale < d->rows)
+        return B200_ERR_PARAM;
+    if (!aligned16(d->x) || !aligned16(d->q)) return B200_ERR_PARAM;
+    if (d->rows > (1ll << 31) - 1 || d->K > (1ll << 24)) return B200_ERR_UNSUPPORTED;
+    if (d->rows == 0) return B200_OK;
+    const int sms = lin::device_sm_count();
+    if (sms <= 0) return B200_ERR_NOT_SM100;
+    const int blocks = static_cast<int>((d->K + fp8::kBlock - 1) / fp8::kBlock);
+    const long long items = d->rows * blocks;
+    long long ctas = (items + 31) / 32;
+    const long long most = static_cast<long long>(sms) * 8;
+    if (ctas > most) ctas = most;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const dim3 grid(static_cast<unsigned>(ctas));
+    if (d->x_dtype == B200_F16) launch_kernel(quantize_fp8_kernel<B200_F16>, grid, dim3(256), 0, stream, *d, items, blocks);
+    else if (d->x_dtype == B200_BF16) launch_kernel(quantize_fp8_kernel<B200_BF16>, grid, dim3(256), 0, stream, *d, items, blocks);
+    else launch_kernel(quantize_fp8_kernel<B200_F32>, grid, dim3(256), 0, stream, *d, items, blocks);
+    count_launch();
+    return check_launch();
+}
+
+int b200_add_layernorm_fp8_fwd(const B200LayerNormFp8Desc* d, b200_stream_t stream_) {
+    using namespace b200;
+    if (!d || !d->x || !d->q || !d->scale || !d->gamma || !d->beta) return B200_ERR_PARAM;
+    if (d->rows < 0 || d->H <= 0 || !is_half_dtype(d->dtype)) return B200_ERR_PARAM;
+    if ((d->H % 16) || (d->ldx % 8) || (d->ldq % 16) || d->ldx < d->H || d->ldq < d->H || d->ld_scale < d->rows)
+        return B200_ERR_PARAM;
+    if (d->residual && ((d->ldr % 8) || d->ldr < d->H || !aligned16(d->residual))) return B200_ERR_PARAM;
+    if (d->y && ((d->ldy % 8) || d->ldy < d->H || !aligned16(d->y))) return B200_ERR_PARAM;
+    if (!aligned16(d->x) || !aligned16(d->q) || !aligned16(d->gamma) || !aligned16(d->beta)) return B200_ERR_PARAM;
+    if (d->H > 4096 || d->rows > (1ll << 31) - 1) return B200_ERR_UNSUPPORTED;
+    if (d->rows == 0) return B200_OK;
+    const int sms = lin::device_sm_count();
+    if (sms <= 0) return B200_ERR_NOT_SM100;
+    const int nv = static_cast<int>((d->H / 8 + 31) / 32);
+    const int per_sm = nv <= 1 ? 6 : (nv <= 4 ? 3 : (nv <= 8 ? 2 : 1));
+    long long ctas = (d->rows + 7) / 8;
+    if (ctas > static_cast<long long>(sms) * per_sm) ctas = static_cast<long long>(sms) * per_sm;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (d->dtype == B200_F16) choose_layernorm_fp8<B200_F16>(nv, static_cast<unsigned>(ctas), stream, *d);
+    else choose_layernorm_fp8<B200_BF16>(nv, static_cast<unsigned>(ctas), stream, *d);
+    count_launch();
+    return check_launch();
+}
+
+int b200_pack_weight_fp8(const float* w_kn, int64_t K, int64_t N, int64_t ld_src, void* w_nk, int64_t ld_dst, float* w_scale,
+                         b200_stream_t stream_) {
+    using namespace b200;
+    if (!w_kn || !w_nk || !w_scale || K <= 0 || N <= 0 || ld_src < N || ld_dst < K || (K % 16) || (ld_dst % 16) || !aligned16(w_nk))
+        return B200_ERR_PARAM;
+    if (K > (1ll << 24) || N > 65535ll * 128) return B200_ERR_UNSUPPORTED;
+    if (lin::device_sm_count() <= 0) return B200_ERR_NOT_SM100;
+    const int kblocks = static_cast<int>((K + 127) / 128);
+    const dim3 grid(static_cast<unsigned>(kblocks), static_cast<unsigned>((N + 127) / 128));
+    pack_weight_fp8_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream_)>>>(w_kn, K, N, ld_src, static_cast<uint8_t*>(w_nk),
+                                                                               ld_dst, w_scale, kblocks);
+    count_launch();
+    return check_launch();
+}
+
+}  // extern "C"

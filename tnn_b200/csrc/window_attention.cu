@@ -1,0 +1,609 @@
+// Sliding-window attention with first tokens that stay visible, head_dim 64, grouped key / value heads:
+//   out_i = sum_j p_ij v_j,  p_i = softmax over { j < kv_len : j < sinks or pos_i - left <= j <= pos_i + right } of scale q_i.k_j + mask_j.
+//
+// The keys that a block of 128 queries can see are at most two runs: the first tokens [0, sinks) and the window
+// [p_first - left, p_last + right], one run where they touch.  An item (128 queries of one head of one sequence) walks the
+// runs in tiles of up to 128 keys that start where the run starts, not at multiples of 128; the last tile of a run is as
+// short as the run needs, in steps of 32 keys (QK^T with N = 32 c, PV with K = 32 c, c chunks of softmax), so that four sinks
+// cost a quarter of a tile.
+//
+// tcgen05 (S = Q K^T, O += P V), one softmax warpgroup, online softmax with lazy maximum; persistent CTAs, two per SM, so
+// that one's exp pass covers the other's hand-offs.
+#include "common.cuh"
+#include "linear_common.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int HD = 64;                       // head dimension
+constexpr int TQ = 128;                      // queries per item
+constexpr int TK = 128;                      // keys per tile at most
+constexpr int TILE_BYTES = 128 * HD * 2;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazyLog2 = 8.0f;            // the running maximum moves only when a tile exceeds it by more than 2^8
+
+__device__ __forceinline__ float fast_exp2(float x) {   // one MUFU instruction, 0 below the normal range
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct WindowParams {
+    const float* mask_add;
+    const int* kv_len;
+    const int* q_start;
+    void* out;
+    int Sq, Sk, heads, group;           // group = heads / kv_heads
+    long long ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch;
+    int left, right;                    // both clamped to kUnlimited where there is no limit
+    int sinks;
+    float scale_log2, mask_below;
+    uint32_t idesc_qk, idesc_pv;        // idesc_qk without its N field
+    unsigned int* status;
+    int n_qb, n_items;
+};
+constexpr int kUnlimited = 1 << 28;          // beyond every position (Sq, Sk <= 2^24, q_start clamped to +-2^26)
+
+// The keys that queries at positions [p_first, p_last] of a sequence can see, as runs [0, a_end) and [b_lo, b_hi).
+struct Runs {
+    int a_end, b_lo, b_hi;
+};
+__device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int p_first, int p_last) {
+    Runs r;
+    r.a_end = min(p.sinks, kv);
+    r.b_lo = max(0, p_first - p.left);
+    r.b_hi = min(kv, p_last + p.right + 1);
+    if (r.b_hi <= r.b_lo) {                  // nothing but the first tokens
+        r.b_lo = r.b_hi = 0;
+    } else if (r.b_lo <= r.a_end) {          // the runs touch
+        r.b_lo = 0;
+        r.b_hi = max(r.b_hi, r.a_end);
+        r.a_end = 0;
+    }
+    return r;
+}
+__device__ __forceinline__ int sequence_keys(const WindowParams& p, int b) {
+    if (p.kv_len == nullptr) return p.Sk;
+    return min(max(p.kv_len[b], 0), p.Sk);
+}
+__device__ __forceinline__ int first_position(const WindowParams& p, int b) {
+    if (p.q_start == nullptr) return 0;
+    return min(max(p.q_start[b], -(1 << 26)), 1 << 26);
+}
+// bits [0, n) of a word, n clamped to [0, 32]
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+
+// ---------------------------------------------------------------------------------------------------------------
+// Roles (256 threads, two CTAs per SM; registers move from the control warpgroup to the softmax warpgroup):
+//   warp 0     : producer, TMA loads of Q (two sets: this item's, the next one's) and of K / V tiles through a 2-stage ring,
+//                and with a mask the tile's 128 additive values and visible bits;
+//   warp 1     : UMMA issuer (one elected lane): S(j + 1) before PV(j), across items;
+//   warp 2     : zeroes the V rows of a tile that no query may see (beyond the run, or dropped by the mask): their weight is
+//                exactly 0, but 0 x NaN is not;
+//   warps 4..7 : softmax, thread = query row.
+// TMEM: S 128 columns, O 64, P 64 (half precision, the A operand of PV).
+struct WCfg {
+    static constexpr int THREADS = 256;
+    static constexpr int REGS_CONTROL = 64, REGS_SOFTMAX = 192;
+    static constexpr int NST = 2;
+    static constexpr int OFF_Q = 0;
+    static constexpr int OFF_K = 2 * TILE_BYTES;
+    static constexpr int OFF_V = OFF_K + NST * TILE_BYTES;
+    static constexpr int OFF_MASK = OFF_V + NST * TILE_BYTES;      // NST x 128 floats
+    static constexpr int OFF_BITS = OFF_MASK + NST * TK * 4;       // NST x 4 words
+    static constexpr int OFF_BAR = OFF_BITS + NST * 16;
+    static constexpr int SMEM = OFF_BAR + 256;
+    static constexpr int TMEM_COLS = 256, COL_O = 128, COL_P = 192;
+};
+static_assert(128 * WCfg::REGS_CONTROL + 128 * WCfg::REGS_SOFTMAX <= 65536 / 2, "setmaxnreg moves registers inside the CTA's own share");
+
+struct WItem {
+    int b, head, q0, p0;      // p0: position of the item's first query
+    int a_end, b_lo, b_hi;
+    int n_a, n;               // tiles of the first run, of both
+};
+struct WTile {
+    int k0, end, chunks;      // first key, end of its run, 32-key chunks
+};
+
+__device__ __forceinline__ WItem load_item(const WindowParams& p, int id) {
+    WItem it;
+    // heads fastest: the heads of a group read the same keys and values
+    it.head = id % p.heads;
+    const int rest = id / p.heads;
+    it.q0 = (rest % p.n_qb) * TQ;
+    it.b = rest / p.n_qb;
+    it.p0 = first_position(p, it.b) + it.q0;
+    const Runs r = visible_runs(p, sequence_keys(p, it.b), it.p0, it.p0 + min(TQ, p.Sq - it.q0) - 1);
+    it.a_end = r.a_end;
+    it.b_lo = r.b_lo;
+    it.b_hi = r.b_hi;
+    it.n_a = (r.a_end + TK - 1) / TK;
+    it.n = it.n_a + (r.b_hi - r.b_lo + TK - 1) / TK;
+    return it;
+}
+__device__ __forceinline__ WTile load_tile(const WItem& it, int j) {
+    WTile t;
+    t.k0 = j < it.n_a ? j * TK : it.b_lo + (j - it.n_a) * TK;
+    t.end = j < it.n_a ? it.a_end : it.b_hi;
+    t.chunks = (min(TK, t.end - t.k0) + 31) >> 5;
+    return t;
+}
+
+// MASKED: with an additive key mask
+template <int DT, bool MASKED>
+__global__ void __launch_bounds__(WCfg::THREADS, 2)
+window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const WindowParams p) {
+    using C = WCfg;
+    constexpr int NST = C::NST;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* q_full = bars;                 // [2]
+    uint64_t* q_free = q_full + 2;           // [2] the item's last QK^T has read its queries
+    uint64_t* k_full = q_free + 2;           // [NST]
+    uint64_t* v_full = k_full + NST;
+    uint64_t* v_ready = v_full + NST;        // the rows that nobody may see are zero
+    uint64_t* k_empty = v_ready + NST;
+    uint64_t* v_empty = k_empty + NST;
+    uint64_t* m_full = v_empty + NST;        // mask values and bits written (32 arrivals)
+    uint64_t* s_full = m_full + NST;
+    uint64_t* s_free = s_full + 1;           // the scores are in registers (128 arrivals)
+    uint64_t* p_full = s_free + 1;           // 128 arrivals
+    uint64_t* o_full = p_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    float* mask_s = reinterpret_cast<float*>(smem + C::OFF_MASK);
+    uint32_t* bits_s = reinterpret_cast<uint32_t*>(smem + C::OFF_BITS);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if ((smem_u32(smem) & 1023u) != 0) {
+        if (tid == 0 && p.status) atomicOr(p.status, 4u);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_free[i], 1);
+        }
+        for (int i = 0; i < NST; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_ready[i], 32);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&m_full[i], 32);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(s_free, 128);
+        mbar_init(p_full, 128);
+        mbar_init(o_full, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait();   // q, k, v, kv_len and q_start come from earlier kernels; the output may still be read by one
+
+    const int id0 = blockIdx.x, id_step = gridDim.x;
+    constexpr bool masked = MASKED;
+    // Items without a visible key have no tiles: only the softmax warpgroup, which writes their zeros, stops at them.  `k`
+    // counts the others (query set and phase), `t` tiles (ring stage and phase).
+    if (warp < 4) {
+        setmaxnreg_dec<C::REGS_CONTROL>();
+        if (warp == 0) {
+            // ------------------------------------------------------------ producer
+            bool ok = true;
+            uint32_t k = 0, t = 0;
+            for (int id = id0; ok && id < p.n_items; id += id_step) {
+                const WItem it = load_item(p, id);
+                if (it.n == 0) continue;
+                const int kv_col = it.head / p.group * HD;
+                const uint32_t set = k & 1u;
+                if (!mbar_wait(&q_free[set], ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                if (lane == 0) {
+                    mbar_expect_tx(&q_full[set], TILE_BYTES);
+                    tma_load_3d(smem + C::OFF_Q + set * TILE_BYTES, &tm_q, &q_full[set], it.head * HD, it.q0, it.b);
+                }
+                ++k;
+                for (int j = 0; j < it.n; ++j, ++t) {
+                    const WTile tl = load_tile(it, j);
+                    const int st = static_cast<int>(t % NST);
+                    const uint32_t ph = ((t / NST) & 1u) ^ 1u;
+                    if (!mbar_wait(&k_empty[st], ph, abort_flag)) { ok = false; break; }
+                    if (lane == 0) {
+                        mbar_expect_tx(&k_full[st], TILE_BYTES);
+                        tma_load_3d(smem + C::OFF_K + st * TILE_BYTES, &tm_k, &k_full[st], kv_col, tl.k0, it.b);
+                    }
+                    if (!mbar_wait(&v_empty[st], ph, abort_flag)) { ok = false; break; }   // also: the stage's mask is done with
+                    if (lane == 0) {
+                        mbar_expect_tx(&v_full[st], TILE_BYTES);
+                        tma_load_3d(smem + C::OFF_V + st * TILE_BYTES, &tm_v, &v_full[st], kv_col, tl.k0, it.b);
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int key = tl.k0 + c * 32 + lane;
+                            float m = 0.f;
+                            bool seen = false;
+                            if (key < tl.end) {
+                                m = p.mask_add[static_cast<long long>(it.b) * p.Sk + key];
+                                seen = m > p.mask_below;
+                            }
+                            mask_s[st * TK + c * 32 + lane] = seen ? m * kLog2e : 0.f;
+                            const uint32_t word = __ballot_sync(0xffffffffu, seen);
+                            if (lane == 0) bits_s[st * 4 + c] = word;
+                        }
+                        mbar_arrive(&m_full[st]);
+                    }
+                }
+            }
+            if (!ok && lane == 0) {
+                for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ UMMA issuer
+            if (elect_one()) {
+                const uint64_t dq0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_Q));
+                const uint64_t dk0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_K));
+                const uint64_t dv0 = make_smem_desc_sw128(smem_u32(smem + C::OFF_V));
+                uint32_t n_s = 0, n_pv = 0;   // QK^T and PV issued so far
+                // S of tile j of the CTA's k-th item, once the softmax has taken the scores in front of it
+                auto issue_s = [&](const WItem& it, int j, uint32_t k) -> bool {
+                    const int st = static_cast<int>(n_s % NST);
+                    if (j == 0 && !mbar_wait(&q_full[k & 1u], (k >> 1) & 1u, abort_flag)) return false;
+                    if (!mbar_wait(&k_full[st], (n_s / NST) & 1u, abort_flag)) return false;
+                    if (!mbar_wait(s_free, (n_s & 1u) ^ 1u, abort_flag)) return false;
+                    tcgen05_fence_after();
+                    const uint32_t idesc = p.idesc_qk | (static_cast<uint32_t>(load_tile(it, j).chunks * 4) << 17);
+                    const uint64_t a = dq0 + static_cast<uint64_t>((k & 1u) * (TILE_BYTES >> 4));
+                    const uint64_t b = dk0 + static_cast<uint64_t>(st * (TILE_BYTES >> 4));
+#pragma unroll
+                    for (int e = 0; e < HD / 16; ++e) umma_f16_ss(tmem_base, a + 2u * e, b + 2u * e, idesc, e != 0 ? 1u : 0u);
+                    umma_commit(s_full);
+                    umma_commit(&k_empty[st]);
+                    if (j == it.n - 1) umma_commit(&q_free[k & 1u]);
+                    ++n_s;
+                    return true;
+                };
+                auto issue_pv = [&](const WItem& it, int j) -> bool {
+                    const int st = static_cast<int>(n_pv % NST);
+                    if (!mbar_wait(&v_ready[st], (n_pv / NST) & 1u, abort_flag)) return false;
+                    if (!mbar_wait(p_full, n_pv & 1u, abort_flag)) return false;
+                    tcgen05_fence_after();
+                    const int steps = load_tile(it, j).chunks * 2;
+                    const uint64_t b = dv0 + static_cast<uint64_t>(st * (TILE_BYTES >> 4));
+                    for (int e = 0; e < steps; ++e)   // P: 8 columns per 16 keys, V: 2 KB per 16 keys
+                        umma_f16_ts(tmem_base + C::COL_O, tmem_base + C::COL_P + e * 8, b + static_cast<uint64_t>(e * (2048 >> 4)),
+                                    p.idesc_pv, (j | e) != 0 ? 1u : 0u);
+                    umma_commit(o_full);
+                    umma_commit(&v_empty[st]);
+                    ++n_pv;
+                    return true;
+                };
+                auto next = [&](int id, WItem& it) -> int {   // the first item at or after `id` that has tiles
+                    for (; id < p.n_items; id += id_step) {
+                        it = load_item(p, id);
+                        if (it.n != 0) return id;
+                    }
+                    return id;
+                };
+                WItem it, it_n;
+                uint32_t k = 0;
+                int id = next(id0, it);
+                bool ok = id >= p.n_items || issue_s(it, 0, k);
+                while (ok && id < p.n_items) {
+                    const int id_n = next(id + id_step, it_n);
+                    for (int j = 0; ok && j < it.n; ++j) {
+                        if (j + 1 < it.n) ok = issue_s(it, j + 1, k);
+                        else if (id_n < p.n_items) ok = issue_s(it_n, 0, k + 1);
+                        ok = ok && issue_pv(it, j);
+                    }
+                    id = id_n;
+                    it = it_n;
+                    ++k;
+                }
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // ------------------------------------------------------------ V rows that nobody may see
+            bool ok = true;
+            uint32_t t = 0;
+            for (int id = id0; ok && id < p.n_items; id += id_step) {
+                const WItem it = load_item(p, id);
+                for (int j = 0; j < it.n; ++j, ++t) {
+                    const WTile tl = load_tile(it, j);
+                    const int st = static_cast<int>(t % NST);
+                    const uint32_t ph = (t / NST) & 1u;
+                    if (!mbar_wait(&v_full[st], ph, abort_flag)) { ok = false; break; }
+                    if (masked && !mbar_wait(&m_full[st], ph, abort_flag)) { ok = false; break; }
+                    __syncwarp();
+                    const int there = tl.end - tl.k0;
+                    if (masked || there < tl.chunks * 32) {
+                        uint8_t* v = smem + C::OFF_V + st * TILE_BYTES;
+                        for (int c = 0; c < tl.chunks; ++c) {
+                            uint32_t hide = ~low_bits(there - c * 32);
+                            if (masked) hide |= ~bits_s[st * 4 + c];
+                            while (hide != 0) {   // four rows of 128 bytes at a time, 8 lanes each (zeros need no swizzle)
+                                uint32_t rest = hide;
+                                int row = -1;
+                                for (int i = 0; i < 4 && rest != 0; ++i) {
+                                    if (i == (lane >> 3)) row = __ffs(rest) - 1;
+                                    rest &= rest - 1u;
+                                }
+                                if (row >= 0)
+                                    *reinterpret_cast<uint4*>(v + (c * 32 + row) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                                hide = rest;
+                            }
+                        }
+                        fence_async_proxy_shared();   // the UMMA reads shared memory through the async proxy
+                    }
+                    mbar_arrive(&v_ready[st]);
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        setmaxnreg_inc<C::REGS_SOFTMAX>();
+        // ------------------------------------------------------------ softmax
+        const int r_in_tile = tid - 128;
+        const uint32_t t_s = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t t_o = t_s + C::COL_O, t_p = t_s + C::COL_P;
+        uint32_t t = 0;
+        bool ok = true;
+        for (int id = id0; ok && id < p.n_items; id += id_step) {
+            const WItem it = load_item(p, id);
+            const int rows = min(TQ, p.Sq - it.q0);
+            const int pos = it.p0 + r_in_tile;
+            const int kv_lo = pos - p.left, kv_hi = pos + p.right;   // the row's window
+            float m_run = -INFINITY, l_run = 0.f;
+            for (int j = 0; j < it.n; ++j, ++t) {
+                const WTile tl = load_tile(it, j);
+                const int st = static_cast<int>(t % NST);
+                // every key of the tile visible to every row
+                const bool plain = !masked && p.scale_log2 > 0.f && tl.end - tl.k0 >= TK &&
+                                   (tl.k0 + TK <= p.sinks || (tl.k0 >= it.p0 + rows - 1 - p.left && tl.k0 + TK - 1 <= it.p0 + p.right));
+                if (masked && !mbar_wait(&m_full[st], (t / NST) & 1u, abort_flag)) { ok = false; break; }
+                if (!mbar_wait(s_full, t & 1u, abort_flag)) { ok = false; break; }
+                __syncwarp();
+                tcgen05_fence_after();
+                uint32_t s[TK];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < tl.chunks) tmem_ld_32x32b_x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < tl.chunks) tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+                tcgen05_fence_before();
+                mbar_arrive(s_free);
+                float tmx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (plain) {
+#pragma unroll
+                    for (int g = 0; g < TK / 8; ++g) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            tmx[c] = fmax3(tmx[c], __uint_as_float(s[g * 8 + c * 2]), __uint_as_float(s[g * 8 + c * 2 + 1]));
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c < tl.chunks) {
+                            const int k0 = tl.k0 + c * 32;
+                            uint32_t bits = (low_bits(kv_hi + 1 - k0) & ~low_bits(kv_lo - k0)) | low_bits(p.sinks - k0);
+                            bits &= low_bits(tl.end - k0);
+                            if (masked) {
+                                bits &= bits_s[st * 4 + c];
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    const float x = fmaf(__uint_as_float(s[c * 32 + e]), p.scale_log2, mask_s[st * TK + c * 32 + e]);
+                                    s[c * 32 + e] = __float_as_uint((bits >> e) & 1u ? x : -INFINITY);
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    const float x = __uint_as_float(s[c * 32 + e]) * p.scale_log2;
+                                    s[c * 32 + e] = __float_as_uint((bits >> e) & 1u ? x : -INFINITY);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2)
+                                tmx[(e >> 1) & 3] = fmax3(tmx[(e >> 1) & 3], __uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1]));
+                        }
+                    }
+                }
+                float tmax = fmaxf(fmaxf(tmx[0], tmx[1]), fmaxf(tmx[2], tmx[3]));
+                if (plain) tmax *= p.scale_log2;
+                const bool move = tmax > m_run + kLazyLog2;
+                const float m_new = move ? tmax : m_run;
+                const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+                const float alpha = move ? fast_exp2(m_run - m_use) : 1.f;
+                // PV of the item's previous tile is complete: it read the P columns and wrote the accumulator
+                if (j > 0 && !mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
+                __syncwarp();
+                if (j > 0 && __any_sync(0xffffffffu, move)) {
+                    tcgen05_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {   // 16 columns at a time: the scores occupy most registers
+                        uint32_t ro[16];
+                        tmem_ld_32x32b_x16(t_o + c * 16, ro);
+                        tmem_ld_wait(ro);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) ro[e] = __float_as_uint(__uint_as_float(ro[e]) * alpha);
+                        tmem_st_32x32b_x16(t_o + c * 16, ro);
+                    }
+                }
+                const float mul = plain ? p.scale_log2 : 1.f;
+                const uint64_t mul2 = pack_f32x2(mul, mul), neg2 = pack_f32x2(-m_use, -m_use);
+                uint64_t ps2[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c < tl.chunks) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int i = c * 32 + e * 2;
+                            float x0, x1;
+                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), mul2, neg2), x0, x1);
+                            x0 = fast_exp2(x0);
+                            x1 = fast_exp2(x1);
+                            ps2[e & 1] = add_f32x2(ps2[e & 1], pack_f32x2(x0, x1));
+                            pk[e] = pack2t<DT>(x0, x1);
+                        }
+                        tmem_st_32x32b_x16(t_p + c * 16, pk);
+                    }
+                }
+                float a0, a1, a2, a3;
+                unpack_f32x2(ps2[0], a0, a1);
+                unpack_f32x2(ps2[1], a2, a3);
+                l_run = l_run * alpha + ((a0 + a1) + (a2 + a3));
+                m_run = m_new;
+                tmem_st_wait();
+                tcgen05_fence_before();
+                mbar_arrive(p_full);
+            }
+            if (!ok) break;
+            if (it.n > 0 && !mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
+            __syncwarp();
+            tcgen05_fence_after();
+            // l_run is 0 where no key was visible (a sum of weights is at least the maximum's 2^-8), NaN where a score was
+            const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+            const int q = it.q0 + r_in_tile;
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_batch + q * p.ldo + it.head * HD;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t r[32];
+                if (it.n > 0) {
+                    tmem_ld_32x32b_x32(t_o + c * 32, r);
+                    tmem_ld_wait(r);
+                }
+                if (q < p.Sq) {
+                    const bool none = it.n == 0 || l_run == 0.f;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint4 qv;
+                        qv.x = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 0]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
+                        qv.y = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
+                        qv.z = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
+                        qv.w = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
+                        *reinterpret_cast<uint4*>(dst + c * 32 + g * 8) = qv;
+                    }
+                }
+            }
+            tcgen05_fence_before();
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    if (tid == 0 && *abort_flag != 0 && p.status != nullptr) atomicOr(p.status, 2u);
+}
+
+bool set_window_attributes(int dev) {
+    static PerDeviceOnce once;
+    return once.ensure(dev, []() {
+        auto set = [](const void* f) {
+            return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, WCfg::SMEM) == cudaSuccess;
+        };
+        return set(reinterpret_cast<const void*>(window_attention_kernel<B200_F16, false>)) &&
+               set(reinterpret_cast<const void*>(window_attention_kernel<B200_F16, true>)) &&
+               set(reinterpret_cast<const void*>(window_attention_kernel<B200_BF16, false>)) &&
+               set(reinterpret_cast<const void*>(window_attention_kernel<B200_BF16, true>));
+    });
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_stream_t stream_) {
+    using namespace b200;
+    if (!d || !d->q || !d->k || !d->v || !d->out) return B200_ERR_PARAM;
+    if (d->B < 0 || d->Sq < 0 || d->Sk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads || d->sinks < 0)
+        return B200_ERR_PARAM;
+    if (d->head_dim != HD) return B200_ERR_UNSUPPORTED;
+    if (!is_half_dtype(d->dtype)) return B200_ERR_PARAM;
+    const int64_t wq = static_cast<int64_t>(d->heads) * HD, wk = static_cast<int64_t>(d->kv_heads) * HD;
+    if ((d->ldq % 8) || (d->ldk % 8) || (d->ldv % 8) || (d->ldo % 8)) return B200_ERR_PARAM;
+    if ((d->q_batch % 8) || (d->k_batch % 8) || (d->v_batch % 8) || (d->o_batch % 8)) return B200_ERR_PARAM;
+    if (d->ldq < wq || d->ldk < wk || d->ldv < wk || d->ldo < wq) return B200_ERR_PARAM;
+    if (d->B > 1 && (d->q_batch <= 0 || d->k_batch <= 0 || d->v_batch <= 0 || d->o_batch < (d->Sq - 1) * d->ldo + wq))
+        return B200_ERR_PARAM;
+    if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out)) return B200_ERR_PARAM;
+    if (d->B > 65535 || d->heads > 65535 || d->Sq > (1 << 24) || d->Sk > (1 << 24)) return B200_ERR_UNSUPPORTED;
+    if (d->B == 0 || d->Sq == 0) return B200_OK;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return B200_ERR_LAUNCH;
+    const int sms = lin::device_sm_count();
+    if (sms <= 0) return B200_ERR_NOT_SM100;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+
+    WindowParams p;
+    p.mask_add = d->mask_add;
+    p.kv_len = d->kv_len;
+    p.q_start = d->q_start;
+    p.out = d->out;
+    p.Sq = static_cast<int>(d->Sq);
+    p.Sk = static_cast<int>(d->Sk);
+    p.heads = d->heads;
+    p.group = d->heads / d->kv_heads;
+    p.ldq = d->ldq;
+    p.ldk = d->ldk;
+    p.ldv = d->ldv;
+    p.ldo = d->ldo;
+    const bool many = d->B > 1;   // one sequence: the batch strides mean nothing
+    p.q_batch = many ? d->q_batch : d->Sq * d->ldq;
+    p.k_batch = many ? d->k_batch : d->Sk * d->ldk;
+    p.v_batch = many ? d->v_batch : d->Sk * d->ldv;
+    p.o_batch = many ? d->o_batch : d->Sq * d->ldo;
+    auto side = [](int64_t w) { return w < 0 || w > kUnlimited ? kUnlimited : static_cast<int>(w); };
+    p.left = side(d->left);
+    p.right = side(d->right);
+    p.sinks = d->sinks > d->Sk ? p.Sk : static_cast<int>(d->sinks);
+    p.scale_log2 = d->scale * kLog2e;
+    p.mask_below = d->mask_exclude_below;
+    p.status = device_status_ptr();
+
+    const long long n_qb = (d->Sq + TQ - 1) / TQ;
+    const long long items = n_qb * d->heads * d->B;
+    if (items > 0x7fff0000ll) return B200_ERR_UNSUPPORTED;
+    p.n_qb = static_cast<int>(n_qb);
+    p.n_items = static_cast<int>(items);
+    const int fmt = d->dtype == B200_BF16 ? 1 : 0;
+    p.idesc_qk = make_idesc_f16(TQ, 0, fmt, 0, 0);
+    p.idesc_pv = make_idesc_f16(TQ, HD, fmt, 0, 1);   // V is MN-major
+    const uint32_t box[3] = {HD, 128, 1};
+    const uint64_t B = static_cast<uint64_t>(d->B);
+    const uint64_t qd[3] = {static_cast<uint64_t>(wq), static_cast<uint64_t>(d->Sq), B};
+    const uint64_t kd[3] = {static_cast<uint64_t>(wk), static_cast<uint64_t>(d->Sk), B};
+    const uint64_t qs[2] = {static_cast<uint64_t>(d->ldq) * 2, static_cast<uint64_t>(p.q_batch) * 2};
+    const uint64_t ks[2] = {static_cast<uint64_t>(d->ldk) * 2, static_cast<uint64_t>(p.k_batch) * 2};
+    const uint64_t vs[2] = {static_cast<uint64_t>(d->ldv) * 2, static_cast<uint64_t>(p.v_batch) * 2};
+    CUtensorMap tq, tk, tv;
+    if (!get_tensor_map(&tq, d->q, 3, qd, qs, box) || !get_tensor_map(&tk, d->k, 3, kd, ks, box) ||
+        !get_tensor_map(&tv, d->v, 3, kd, vs, box))
+        return B200_ERR_DRIVER;
+    if (!set_window_attributes(dev)) return B200_ERR_LAUNCH;
+    const long long slots = 2ll * sms;
+    const dim3 grid(static_cast<unsigned>(items < slots ? items : slots));
+    const bool masked = d->mask_add != nullptr;
+    auto kernel = d->dtype == B200_F16 ? (masked ? window_attention_kernel<B200_F16, true> : window_attention_kernel<B200_F16, false>)
+                                       : (masked ? window_attention_kernel<B200_BF16, true> : window_attention_kernel<B200_BF16, false>);
+    launch_kernel(kernel, grid, dim3(WCfg::THREADS), WCfg::SMEM, stream, tq, tk, tv, p);
+    count_launch();
+    return check_launch();
+}
