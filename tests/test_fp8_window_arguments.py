@@ -100,7 +100,7 @@ def launches(monkeypatch):
     """CPU tensors go through the wrappers' checks; what would be launched is recorded."""
     seen = []
     monkeypatch.setattr(ops, "_require_cuda", lambda *ts: None)
-    monkeypatch.setattr(ops, "_call", lambda name, desc, device: seen.append((name, desc)))
+    monkeypatch.setattr(ops, "_call", lambda name, desc, index: seen.append((name, desc)))
     return seen
 
 

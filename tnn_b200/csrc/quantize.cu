@@ -32,54 +32,81 @@ __device__ __forceinline__ void decode16(const Raw16<DT>& r, float (&v)[16]) {
     }
 }
 
+// Largest magnitude of 16 elements, as the bits of an fp32 value (ordered as integers, NaN above infinity).  Half-precision
+// magnitudes are ordered the same way, so two at a time are compared before one is widened.
 template <int DT>
-__global__ void __launch_bounds__(256) quantize_fp8_kernel(B200QuantizeFp8Desc d, long long items, int blocks) {
+__device__ __forceinline__ uint32_t amax_bits16(const Raw16<DT>& r) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < Raw16<DT>::Q; ++i) {
+        const uint32_t w[4] = {r.q[i].x, r.q[i].y, r.q[i].z, r.q[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (DT == B200_F32) m = max(m, w[e] & 0x7FFFFFFFu);
+            else m = __vmaxu2(m, w[e] & 0x7FFF7FFFu);
+        }
+    }
+    if constexpr (DT == B200_F32) return m;
+    m = max(m & 0xFFFFu, m >> 16);
+    return __float_as_uint(unpack2(m, DT).x);
+}
+
+// An item is a block of one row.  Items are dealt to the groups of all CTAs in turn; a group finds the row and block of its
+// next item from those of the last one (a 64-bit division per item took as long as the item's bytes: 65536 x 1024 bf16
+// 64.6 us).
+template <int DT>
+__global__ void __launch_bounds__(256) quantize_fp8_kernel(B200QuantizeFp8Desc d, int blocks) {
     constexpr int UNROLL = DT == B200_F32 ? 2 : 4;
     constexpr int kGroups = 32;   // blocks of 128 values per CTA and step
     pdl_launch_dependents();
     pdl_wait();
-    const int group = threadIdx.x >> 3, sub = threadIdx.x & 7;
-    const long long step = static_cast<long long>(gridDim.x) * kGroups;
-    for (long long i0 = static_cast<long long>(blockIdx.x) * kGroups + group; i0 - group < items; i0 += step * UNROLL) {
+    const int sub = threadIdx.x & 7;
+    const unsigned step = gridDim.x * kGroups, first = blockIdx.x * kGroups + (threadIdx.x >> 3);
+    const int step_rows = static_cast<int>(step / blocks), step_blocks = static_cast<int>(step % blocks);
+    long long row = first / blocks;
+    int kb = static_cast<int>(first % blocks);
+    while (__any_sync(0xffffffffu, row < d.rows)) {
         Raw16<DT> raw[UNROLL];
-        bool in[UNROLL];
+        long long rows[UNROLL];
+        int kbs[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const long long i = i0 + u * step;
-            const long long row = i / blocks;
-            const long long col = (i - row * blocks) * fp8::kBlock + sub * 16;
-            in[u] = i < items && col < d.K;
+            rows[u] = row;
+            kbs[u] = kb;
+            const long long col = kb * fp8::kBlock + sub * 16;
 #pragma unroll
             for (int k = 0; k < Raw16<DT>::Q; ++k) raw[u].q[k] = make_uint4(0, 0, 0, 0);
-            if (in[u]) {
+            if (row < d.rows && col < d.K) {
                 const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(d.x) +
                                                                 (row * d.ldx + col) * (DT == B200_F32 ? 4 : 2));
 #pragma unroll
                 for (int k = 0; k < Raw16<DT>::Q; ++k) raw[u].q[k] = __ldg(p + k);
             }
+            row += step_rows;
+            kb += step_blocks;
+            if (kb >= blocks) {
+                kb -= blocks;
+                ++row;
+            }
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const long long i = i0 + u * step;
-            const long long row = i / blocks;
-            const int kb = static_cast<int>(i - row * blocks);
             float v[16];
             decode16<DT>(raw[u], v);
-            uint32_t bits = 0;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) bits = max(bits, fp8::abs_bits(v[e]));
+            uint32_t bits = amax_bits16<DT>(raw[u]);
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
             const float amax = fp8::amax_of_bits(bits);
             const float enc = fp8::encode_scale(amax);
-            if (in[u]) {
+            const int col = kbs[u] * fp8::kBlock + sub * 16;
+            if (rows[u] < d.rows && col < d.K) {
                 uint4 q;
                 q.x = fp8::pack4(v[0] * enc, v[1] * enc, v[2] * enc, v[3] * enc);
                 q.y = fp8::pack4(v[4] * enc, v[5] * enc, v[6] * enc, v[7] * enc);
                 q.z = fp8::pack4(v[8] * enc, v[9] * enc, v[10] * enc, v[11] * enc);
                 q.w = fp8::pack4(v[12] * enc, v[13] * enc, v[14] * enc, v[15] * enc);
-                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(d.q) + row * d.ldq + kb * fp8::kBlock + sub * 16) = q;
-                if (sub == 0) d.scale[kb * d.ld_scale + row] = fp8::decode_scale(amax);
+                *reinterpret_cast<uint4*>(static_cast<uint8_t*>(d.q) + rows[u] * d.ldq + col) = q;
+                if (sub == 0) d.scale[kbs[u] * d.ld_scale + rows[u]] = fp8::decode_scale(amax);
             }
         }
     }
@@ -238,6 +265,8 @@ __global__ void __launch_bounds__(256) pack_weight_fp8_kernel(const float* src, 
     }
 }
 
+constexpr int kQuantizeCtas = 3;   // resident CTAs per SM
+
 template <int NV, int DT>
 void launch_layernorm_fp8(unsigned grid, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
     const size_t smem = static_cast<size_t>(NV) * 256 * 2 * sizeof(float);
@@ -274,15 +303,13 @@ int b200_quantize_fp8(const B200QuantizeFp8Desc* d, b200_stream_t stream_) {
     const int sms = lin::device_sm_count();
     if (sms <= 0) return B200_ERR_NOT_SM100;
     const int blocks = static_cast<int>((d->K + fp8::kBlock - 1) / fp8::kBlock);
-    const long long items = d->rows * blocks;
-    long long ctas = (items + 31) / 32;
-    const long long most = static_cast<long long>(sms) * 8;
-    if (ctas > most) ctas = most;
+    const long long ctas = (d->rows * blocks + 31) / 32;
+    const long long most = static_cast<long long>(sms) * kQuantizeCtas;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    const dim3 grid(static_cast<unsigned>(ctas));
-    if (d->x_dtype == B200_F16) launch_kernel(quantize_fp8_kernel<B200_F16>, grid, dim3(256), 0, stream, *d, items, blocks);
-    else if (d->x_dtype == B200_BF16) launch_kernel(quantize_fp8_kernel<B200_BF16>, grid, dim3(256), 0, stream, *d, items, blocks);
-    else launch_kernel(quantize_fp8_kernel<B200_F32>, grid, dim3(256), 0, stream, *d, items, blocks);
+    const dim3 grid(static_cast<unsigned>(ctas < most ? ctas : most));
+    if (d->x_dtype == B200_F16) launch_kernel(quantize_fp8_kernel<B200_F16>, grid, dim3(256), 0, stream, *d, blocks);
+    else if (d->x_dtype == B200_BF16) launch_kernel(quantize_fp8_kernel<B200_BF16>, grid, dim3(256), 0, stream, *d, blocks);
+    else launch_kernel(quantize_fp8_kernel<B200_F32>, grid, dim3(256), 0, stream, *d, blocks);
     count_launch();
     return check_launch();
 }

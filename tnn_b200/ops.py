@@ -243,33 +243,51 @@ def qa_head(x, weight, bias=None, out=None):
 
 # ---------------------------------------------------------------------------- 8-bit operands with block scales
 FP8_BLOCK = 128   # consecutive values of a row that share a scale
+_F8 = torch.float8_e4m3fn
+_entry = {}       # entry points by name: looking one up in the library object costs more than in a dict
 
 
-def _call(name, desc, device):
-    """Launch `name` on the current stream of the device the tensors are on, whichever device is current."""
-    fn = getattr(capi.lib(), name)
-    if device.index == torch.cuda.current_device():
+def _call(name, desc, index):
+    """Launch `name` on the current stream of device `index`, the one the tensors are on, whichever device is current."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(capi.lib(), name)
+    if index == torch.cuda.current_device():
         rc = fn(ctypes.byref(desc), capi.stream_ptr())
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(ctypes.byref(desc), capi.stream_ptr())
-    capi.check(rc, name)
+    if rc != capi.OK:
+        capi.check(rc, name)
 
 
-def _check(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _same_device(x, *ts):
-    _require_cuda(x, *ts)
+def _device_index(x, *ts):
+    """The one CUDA device of all these tensors."""
+    index = x.get_device()
     for t in ts:
-        _check(t is None or t.device == x.device, "tensors on different devices")
+        if t is not None and t.get_device() != index:
+            raise ValueError("tensors on different devices")
+    if index < 0:
+        _require_cuda(x)
+    return index
+
+
+def _new(shape, dtype, device):
+    """Uninitialised contiguous tensor of two or three dimensions (empty_strided costs 1.5 us of host time, empty 2.4)."""
+    strides = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
+def _new_like(x, dtype):
+    """Uninitialised contiguous tensor of x's shape."""
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=dtype)
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
 
 
 def _vector(t, n, what):
-    _check(t is None or (t.dtype == torch.float32 and t.numel() == n and t.is_contiguous()),
-           "%s: fp32, %d contiguous values" % (what, n))
+    if t is not None and not (t.dtype == torch.float32 and t.numel() == n and t.is_contiguous()):
+        raise ValueError("%s: fp32, %d contiguous values" % (what, n))
 
 
 def _blocks(n):
@@ -278,67 +296,78 @@ def _blocks(n):
 
 def _scale_rows(scale, blocks, rows, what):
     """Row stride of a `[blocks, rows]` fp32 scale array."""
-    _check(scale.dtype == torch.float32 and tuple(scale.shape) == (blocks, rows) and (rows <= 1 or scale.stride(1) == 1),
-           "%s: fp32 [%d, %d] with contiguous rows" % (what, blocks, rows))
-    ld = scale.stride(0) if blocks > 1 else rows
-    _check(ld >= rows, "%s: overlapping rows" % what)
-    return ld
+    if scale.dtype != torch.float32 or scale.shape != (blocks, rows):
+        raise ValueError("%s: fp32 [%d, %d]" % (what, blocks, rows))
+    if scale.is_contiguous():
+        return rows
+    if (rows > 1 and scale.stride(1) != 1) or (blocks > 1 and scale.stride(0) < rows):
+        raise ValueError("%s: contiguous rows that do not overlap" % what)
+    return scale.stride(0) if blocks > 1 else rows
 
 
 def _codes(t, shape, what):
-    _check(t.dtype == torch.float8_e4m3fn and tuple(t.shape) == tuple(shape), "%s: float8_e4m3fn %s" % (what, tuple(shape)))
+    if t.dtype != _F8 or t.shape != shape:
+        raise ValueError("%s: float8_e4m3fn %s" % (what, tuple(shape)))
 
 
 def _out_rows(t, width, rows, what):
-    """`t` as exactly `rows` rows of `width` contiguous elements that the kernel may write: (tensor, row stride).  A view is
+    """`t` as exactly `rows` rows of `width` contiguous elements that the kernel may write: (address, row stride).  A view is
     needed, never a copy: results written to a copy would be lost."""
-    if t.is_contiguous():
-        _check(t.numel() == rows * width, "%s: %d rows of %d" % (what, rows, width))
-        return t, width
-    try:
-        t = t.view(-1, width)
-    except RuntimeError:
-        raise ValueError("%s: cannot be seen as rows of %d without a copy" % (what, width)) from None
-    _check(t.shape[0] == rows and t.stride(1) == 1 and (rows <= 1 or t.stride(0) >= width), "%s: %d rows of %d" % (what, rows, width))
-    return t, t.stride(0)
+    if not t.is_contiguous():
+        try:
+            t = t.view(-1, width)
+        except RuntimeError:
+            raise ValueError("%s: cannot be seen as rows of %d without a copy" % (what, width)) from None
+        if t.shape[0] != rows or t.stride(1) != 1 or (rows > 1 and t.stride(0) < width):
+            raise ValueError("%s: %d rows of %d" % (what, rows, width))
+        return t.data_ptr(), (t.stride(0) if rows > 1 else width)
+    if t.numel() != rows * width:
+        raise ValueError("%s: %d rows of %d" % (what, rows, width))
+    return t.data_ptr(), width
 
 
 def quantize_fp8(x, out=None, out_scale=None):
     """x `[..., K]` (f16, bf16 or f32) -> (codes `[..., K]` float8_e4m3fn, scales fp32 `[ceil(K/128), rows]`).  A value
     stands for code * scale of its row and block of 128 columns (include/tnn_b200.h has the exact rounding)."""
-    _same_device(x, out, out_scale)
+    index = _device_index(x, out, out_scale)
     K = x.shape[-1]
+    blocks = _blocks(K)
     x2, rows, ldx = _rows(x, K)
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    _codes(out, x.shape, "out")
-    q2, ldq = _out_rows(out, K, rows, "out")
+        out = _new_like(x, _F8)
+        q, ldq = out.data_ptr(), K
+    else:
+        _codes(out, x.shape, "out")
+        q, ldq = _out_rows(out, K, rows, "out")
     if out_scale is None:
-        out_scale = torch.empty((_blocks(K), rows), dtype=torch.float32, device=x.device)
-    d = capi.QuantizeFp8Desc(x2.data_ptr(), q2.data_ptr(), out_scale.data_ptr(), rows, K, ldx, ldq,
-                             _scale_rows(out_scale, _blocks(K), rows, "out_scale"), capi.dtype_code(x.dtype))
+        out_scale = _new((blocks, rows), torch.float32, x.device)
+        lds = rows
+    else:
+        lds = _scale_rows(out_scale, blocks, rows, "out_scale")
+    d = capi.QuantizeFp8Desc(x2.data_ptr(), q, out_scale.data_ptr(), rows, K, ldx, ldq, lds, capi.dtype_code(x.dtype))
     if rows:
-        _call("b200_quantize_fp8", d, x.device)
+        _call("b200_quantize_fp8", d, index)
     return out, out_scale
 
 
 def pack_weight_fp8(w_kn, out=None, out_scale=None):
     """fp32 `[K, N]` (TNN MatMul weight layout, y = x.W) -> (codes `[N, K]` float8_e4m3fn, fp32 scales per 128 x 128 block
     `[ceil(N/128), ceil(K/128)]`) for `linear_fp8`."""
-    _same_device(w_kn, out, out_scale)
-    _check(w_kn.dtype == torch.float32 and w_kn.dim() == 2 and w_kn.stride(1) == 1, "w_kn: fp32 [K, N], contiguous columns")
+    index = _device_index(w_kn, out, out_scale)
+    if w_kn.dtype != torch.float32 or w_kn.dim() != 2 or w_kn.stride(1) != 1:
+        raise ValueError("w_kn: fp32 [K, N], contiguous columns")
     K, N = w_kn.shape
     if out is None:
-        out = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=w_kn.device)
-    if out_scale is None:
-        out_scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w_kn.device)
+        out = _new((N, K), _F8, w_kn.device)
     _codes(out, (N, K), "out")
-    _check(out.stride(1) == 1 and out.stride(0) >= K, "out: contiguous rows")
-    _check(out_scale.dtype == torch.float32 and tuple(out_scale.shape) == (_blocks(N), _blocks(K)) and out_scale.is_contiguous(),
-           "out_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
-    with torch.cuda.device(w_kn.device):
-        rc = capi.lib().b200_pack_weight_fp8(w_kn.data_ptr(), K, N, w_kn.stride(0), out.data_ptr(), out.stride(0),
-                                             out_scale.data_ptr(), capi.stream_ptr())
+    w, ldw = _out_rows(out, K, N, "out")
+    if out_scale is None:
+        out_scale = _new((_blocks(N), _blocks(K)), torch.float32, w_kn.device)
+    if out_scale.dtype != torch.float32 or out_scale.shape != (_blocks(N), _blocks(K)) or not out_scale.is_contiguous():
+        raise ValueError("out_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
+    with torch.cuda.device(index):
+        rc = capi.lib().b200_pack_weight_fp8(w_kn.data_ptr(), K, N, w_kn.stride(0) if K > 1 else N, w, ldw, out_scale.data_ptr(),
+                                             capi.stream_ptr())
     capi.check(rc, "b200_pack_weight_fp8")
     return out, out_scale
 
@@ -346,33 +375,41 @@ def pack_weight_fp8(w_kn, out=None, out_scale=None):
 def add_layernorm_fp8(x, gamma, beta, eps, residual=None, out=None, out8=None, out_scale=None, half=True):
     """(residual +) LayerNorm whose result leaves as `(y in x's dtype, codes, scales)`: `add_layernorm` and `quantize_fp8`
     of its fp32 result in one pass.  `half=False`: codes and scales only (y is None)."""
-    _same_device(x, gamma, beta, residual, out, out8, out_scale)
+    index = _device_index(x, gamma, beta, residual, out, out8, out_scale)
     H = x.shape[-1]
+    blocks = _blocks(H)
     _vector(gamma, H, "gamma")
     _vector(beta, H, "beta")
     x2, rows, ldx = _rows(x, H)
-    _check(out is None or half, "out is given but half=False")
-    if out is None and half:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out8 is None:
-        out8 = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    _codes(out8, x.shape, "out8")
-    q2, ldq = _out_rows(out8, H, rows, "out8")
-    if out_scale is None:
-        out_scale = torch.empty((_blocks(H), rows), dtype=torch.float32, device=x.device)
-    d = capi.LayerNormFp8Desc(x2.data_ptr(), None, gamma.data_ptr(), beta.data_ptr(), None, q2.data_ptr(), out_scale.data_ptr(),
-                              rows, H, ldx, 0, 0, ldq, _scale_rows(out_scale, _blocks(H), rows, "out_scale"),
-                              capi.dtype_code(x.dtype), float(eps))
+    y, ldy = None, 0
     if out is not None:
-        _check(out.dtype == x.dtype, "out: the dtype of x")
-        y2, d.ldy = _out_rows(out, H, rows, "out")
-        d.y = y2.data_ptr()
+        if not half or out.dtype != x.dtype:
+            raise ValueError("out: the dtype of x, and none with half=False")
+        y, ldy = _out_rows(out, H, rows, "out")
+    elif half:
+        out = _new_like(x, x.dtype)
+        y, ldy = out.data_ptr(), H
+    if out8 is None:
+        out8 = _new_like(x, _F8)
+        q, ldq = out8.data_ptr(), H
+    else:
+        _codes(out8, x.shape, "out8")
+        q, ldq = _out_rows(out8, H, rows, "out8")
+    if out_scale is None:
+        out_scale = _new((blocks, rows), torch.float32, x.device)
+        lds = rows
+    else:
+        lds = _scale_rows(out_scale, blocks, rows, "out_scale")
+    r, ldr = None, 0
     if residual is not None:
-        _check(residual.dtype == x.dtype, "residual: the dtype of x")
-        r2, _, d.ldr = _rows(residual, H, rows)
-        d.residual = r2.data_ptr()
+        if residual.dtype != x.dtype:
+            raise ValueError("residual: the dtype of x")
+        r2, _, ldr = _rows(residual, H, rows)
+        r = r2.data_ptr()
+    d = capi.LayerNormFp8Desc(x2.data_ptr(), r, gamma.data_ptr(), beta.data_ptr(), y, q, out_scale.data_ptr(), rows, H, ldx, ldr, ldy,
+                              ldq, lds, capi.dtype_code(x.dtype), eps)
     if rows:
-        _call("b200_add_layernorm_fp8_fwd", d, x.device)
+        _call("b200_add_layernorm_fp8_fwd", d, index)
     return out, out8, out_scale
 
 
@@ -381,51 +418,64 @@ def linear_fp8(x8, x_scale, w8, w_scale, bias=None, residual=None, epilogue=EPI_
     """y = epilogue(x . w^T + bias (+ residual)) on block-scaled e4m3 operands: x8 `[..., K]` with x_scale
     `[ceil(K/128), rows]` (`quantize_fp8`), w8 `[N, K]` with w_scale (`pack_weight_fp8`).  `out_dtype` f16, bf16 or f32
     returns y `[..., N]`; float8_e4m3fn returns (codes, scales `[ceil(N/128), rows]`) for another `linear_fp8`."""
-    _same_device(x8, x_scale, w8, w_scale, bias, residual, out, out_scale)
-    K = x8.shape[-1]
-    _check(x8.dtype == torch.float8_e4m3fn and w8.dtype == torch.float8_e4m3fn, "x8, w8: float8_e4m3fn")
-    _check(w8.dim() == 2 and w8.shape[1] == K and w8.stride(1) == 1 and (w8.shape[0] <= 1 or w8.stride(0) >= K),
-           "w8: [N, %d] with contiguous rows" % K)
-    N = w8.shape[0]
-    _check(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (_blocks(N), _blocks(K)) and w_scale.is_contiguous(),
-           "w_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
+    index = _device_index(x8, x_scale, w8, w_scale, bias, residual, out, out_scale)
+    N, K = w8.shape
+    if x8.dtype != _F8 or w8.dtype != _F8 or x8.shape[-1] != K:
+        raise ValueError("x8 [..., K], w8 [N, K]: float8_e4m3fn")
+    if w8.is_contiguous():
+        ldw = K
+    elif w8.stride(1) == 1 and (N <= 1 or w8.stride(0) >= K):
+        ldw = w8.stride(0) if N > 1 else K
+    else:
+        raise ValueError("w8: [N, K] with contiguous rows")
+    if w_scale.dtype != torch.float32 or w_scale.shape != (_blocks(N), _blocks(K)) or not w_scale.is_contiguous():
+        raise ValueError("w_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
     _vector(bias, N, "bias")
     x2, M, ldx = _rows(x8, K)
+    ldxs = _scale_rows(x_scale, _blocks(K), M, "x_scale")
     if out is not None:
         out_dtype = out.dtype
+        y, ldy = _out_rows(out, N, M, "out")
     else:
-        out = torch.empty(x8.shape[:-1] + (N,), dtype=out_dtype, device=x8.device)
-    f8 = out_dtype == torch.float8_e4m3fn
-    y2, ldy = _out_rows(out, N, M, "out")
-    d = capi.LinearFp8Desc(x2.data_ptr(), w8.data_ptr(), x_scale.data_ptr(), w_scale.data_ptr(), capi.ptr(bias), None,
-                           y2.data_ptr(), None, M, N, K, ldx, w8.stride(0) if N > 1 else K, 0, ldy,
-                           _scale_rows(x_scale, _blocks(K), M, "x_scale"), 0,
-                           capi.E4M3 if f8 else capi.dtype_code(out_dtype), capi.F16, epilogue, block_n)
+        out = (_new((M, N), out_dtype, x8.device) if x8.dim() == 2
+               else torch.empty(x8.shape[:-1] + (N,), dtype=out_dtype, device=x8.device))
+        y, ldy = out.data_ptr(), N
+    f8 = out_dtype == _F8
+    ys, ldys = None, 0
     if f8:
         if out_scale is None:
-            out_scale = torch.empty((_blocks(N), M), dtype=torch.float32, device=x8.device)
-        d.ld_y_scale = _scale_rows(out_scale, _blocks(N), M, "out_scale")
-        d.y_scale = out_scale.data_ptr()
+            out_scale = _new((_blocks(N), M), torch.float32, x8.device)
+        ldys = _scale_rows(out_scale, _blocks(N), M, "out_scale")
+        ys = out_scale.data_ptr()
+    r, ldr, r_code = None, 0, capi.F16
     if residual is not None:
-        _check(epilogue == EPI_BIAS_RESIDUAL, "a residual needs epilogue=EPI_BIAS_RESIDUAL")
-        _check(residual.dtype in (torch.float16, torch.bfloat16), "residual: f16 or bf16")
-        r2, _, d.ldr = _rows(residual, N, M)
-        d.residual, d.res_dtype = r2.data_ptr(), capi.dtype_code(residual.dtype)
+        if epilogue != EPI_BIAS_RESIDUAL or residual.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("residual: f16 or bf16, with epilogue=EPI_BIAS_RESIDUAL")
+        r2, _, ldr = _rows(residual, N, M)
+        r, r_code = r2.data_ptr(), capi.dtype_code(residual.dtype)
+    d = capi.LinearFp8Desc(x2.data_ptr(), w8.data_ptr(), x_scale.data_ptr(), w_scale.data_ptr(), capi.ptr(bias), r, y, ys, M, N, K,
+                           ldx, ldw, ldr, ldy, ldxs, ldys, capi.E4M3 if f8 else capi.dtype_code(out_dtype), r_code, epilogue, block_n)
     if M:
-        _call("b200_linear_fp8_fwd", d, x8.device)
+        _call("b200_linear_fp8_fwd", d, index)
     return (out, out_scale) if f8 else out
 
 
 # ---------------------------------------------------------------------------- sliding-window attention
 def _heads_view(t, heads, what):
     """(row stride, batch stride) of a `[B, S, heads * 64]` tensor whose heads lie side by side."""
-    _check(t.dim() == 3 and t.shape[2] == heads * 64 and t.stride(2) == 1, "%s: [B, S, %d], contiguous heads" % (what, heads * 64))
+    if t.dim() != 3 or t.shape[2] != heads * 64:
+        raise ValueError("%s: [B, S, %d]" % (what, heads * 64))
+    if t.is_contiguous():
+        return heads * 64, t.shape[1] * heads * 64
+    if t.stride(2) != 1:
+        raise ValueError("%s: contiguous heads" % what)
     ld = t.stride(1) if t.shape[1] > 1 else heads * 64
     return ld, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * ld)
 
 
 def _per_sequence(t, B, what):
-    _check(t is None or (t.dtype == torch.int32 and t.numel() == B and t.is_contiguous()), "%s: int32 [%d]" % (what, B))
+    if t is not None and not (t.dtype == torch.int32 and t.numel() == B and t.is_contiguous()):
+        raise ValueError("%s: int32 [%d]" % (what, B))
 
 
 def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, mask_add=None, kv_len=None, q_start=None,
@@ -438,31 +488,35 @@ def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, ma
     (None: 0); Sq new tokens at the end of a cache have q_start = kv_len - Sq.  mask_add fp32 `[B, Sk]`: additive key mask, a
     key at or below `exclude_below` is dropped.  A query that sees no key yields zeros; keys and values that no query may see
     (beyond kv_len, or dropped) may hold anything."""
-    kv_heads = heads if kv_heads is None else kv_heads
-    _same_device(q, k, v, mask_add, kv_len, q_start, out)
-    _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, "kv_heads divides heads")
-    _check(q.dtype == k.dtype == v.dtype, "q, k, v: one dtype")
-    _check(sinks >= 0, "sinks >= 0")
+    if kv_heads is None:
+        kv_heads = heads
+    index = _device_index(q, k, v, mask_add, kv_len, q_start, out)
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or sinks < 0:
+        raise ValueError("kv_heads divides heads, sinks >= 0")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError("q, k, v: one dtype")
     ldq, q_batch = _heads_view(q, heads, "q")
     ldk, k_batch = _heads_view(k, kv_heads, "k")
     ldv, v_batch = _heads_view(v, kv_heads, "v")
-    B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
-    _check(k.shape[:2] == v.shape[:2] and k.shape[0] == B, "k, v: [%d, Sk, ...]" % B)
+    B, Sq, _ = q.shape
+    Bk, Sk, _ = k.shape
+    if Bk != B or v.shape != k.shape:
+        raise ValueError("k, v: [%d, Sk, %d]" % (B, kv_heads * 64))
     _per_sequence(kv_len, B, "kv_len")
     _per_sequence(q_start, B, "q_start")
     if out is None:
-        out = torch.empty((B, Sq, heads * 64), dtype=q.dtype, device=q.device)
-    _check(out.dtype == q.dtype and tuple(out.shape) == tuple(q.shape), "out: the dtype and shape of q")
-    ldo, o_batch = _heads_view(out, heads, "out")
-    m2 = None
-    if mask_add is not None:
-        _check(mask_add.dtype == torch.float32 and mask_add.numel() == B * Sk and mask_add.is_contiguous(),
-               "mask_add: contiguous fp32 [%d, %d]" % (B, Sk))
-        m2 = mask_add.data_ptr()
-    d = capi.WindowAttentionDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), m2, capi.ptr(kv_len), capi.ptr(q_start), out.data_ptr(),
-                                 B, Sq, Sk, ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch, window[0], window[1], sinks,
-                                 heads, kv_heads, 64, capi.dtype_code(q.dtype), 0.125 if scale is None else float(scale),
-                                 float(exclude_below))
+        out = _new((B, Sq, heads * 64), q.dtype, q.device)
+        ldo, o_batch = heads * 64, Sq * heads * 64
+    else:
+        if out.dtype != q.dtype or out.shape != q.shape:
+            raise ValueError("out: the dtype and shape of q")
+        ldo, o_batch = _heads_view(out, heads, "out")
+    if mask_add is not None and not (mask_add.dtype == torch.float32 and mask_add.numel() == B * Sk and mask_add.is_contiguous()):
+        raise ValueError("mask_add: contiguous fp32 [%d, %d]" % (B, Sk))
+    d = capi.WindowAttentionDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), capi.ptr(mask_add), capi.ptr(kv_len), capi.ptr(q_start),
+                                 out.data_ptr(), B, Sq, Sk, ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch, window[0],
+                                 window[1], sinks, heads, kv_heads, 64, capi.dtype_code(q.dtype), 0.125 if scale is None else scale,
+                                 exclude_below)
     if B and Sq:
-        _call("b200_window_attention_fwd", d, q.device)
+        _call("b200_window_attention_fwd", d, index)
     return out
