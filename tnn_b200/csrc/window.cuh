@@ -1,0 +1,69 @@
+// What the two window-attention kernels share: the parameters and which keys a run of queries can see.
+#pragma once
+#include "common.cuh"
+
+namespace b200 {
+namespace win {
+
+constexpr int HD = 64;                       // head dimension
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float fast_exp2(float x) {   // one MUFU instruction, 0 below the normal range
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct WindowParams {
+    const float* mask_add;
+    const int* kv_len;
+    const int* q_start;
+    void* out;
+    const void* q;
+    const void* k;
+    const void* v;
+    int Sq, Sk, heads, group;           // group = heads / kv_heads
+    long long ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch;
+    int left, right;                    // both clamped to kUnlimited where there is no limit
+    int sinks;
+    float scale_log2, mask_below;
+    int B;
+    unsigned int* status;
+};
+constexpr int kUnlimited = 1 << 28;          // beyond every position (Sq, Sk <= 2^24, q_start clamped to +-2^26)
+
+// The keys that queries at positions [p_first, p_last] of a sequence can see, as runs [0, a_end) and [b_lo, b_hi).
+struct Runs {
+    int a_end, b_lo, b_hi;
+};
+__device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int p_first, int p_last) {
+    Runs r;
+    r.a_end = min(p.sinks, kv);
+    r.b_lo = max(0, p_first - p.left);
+    r.b_hi = min(kv, p_last + p.right + 1);
+    if (r.b_hi <= r.b_lo) {                  // nothing but the first tokens
+        r.b_lo = r.b_hi = 0;
+    } else if (r.b_lo <= r.a_end) {          // the runs touch
+        r.b_lo = 0;
+        r.b_hi = max(r.b_hi, r.a_end);
+        r.a_end = 0;
+    }
+    return r;
+}
+__device__ __forceinline__ int sequence_keys(const WindowParams& p, int b) {
+    if (p.kv_len == nullptr) return p.Sk;
+    return min(max(p.kv_len[b], 0), p.Sk);
+}
+__device__ __forceinline__ int first_position(const WindowParams& p, int b) {
+    if (p.q_start == nullptr) return 0;
+    return min(max(p.q_start[b], -(1 << 26)), 1 << 26);
+}
+// bits [0, n) of a word, n clamped to [0, 32]
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+
+// A few queries against many keys (window_token.cu): whether it takes this call, and its launch.
+bool token_kernel_takes(const WindowParams& p);
+int launch_window_token(const WindowParams& p, int dtype, int sms, cudaStream_t stream);
+
+}  // namespace win
+}  // namespace b200

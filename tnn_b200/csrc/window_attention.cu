@@ -9,70 +9,23 @@
 //
 // tcgen05 (S = Q K^T, O += P V), one softmax warpgroup, online softmax with lazy maximum; persistent CTAs, two per SM, so
 // that one's exp pass covers the other's hand-offs.
-#include "common.cuh"
 #include "linear_common.cuh"
 #include "ptx.cuh"
+#include "window.cuh"
 
 namespace b200 {
+using namespace win;
 namespace {
 
-constexpr int HD = 64;                       // head dimension
 constexpr int TQ = 128;                      // queries per item
 constexpr int TK = 128;                      // keys per tile at most
 constexpr int TILE_BYTES = 128 * HD * 2;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;            // the running maximum moves only when a tile exceeds it by more than 2^8
 
-__device__ __forceinline__ float fast_exp2(float x) {   // one MUFU instruction, 0 below the normal range
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-struct WindowParams {
-    const float* mask_add;
-    const int* kv_len;
-    const int* q_start;
-    void* out;
-    int Sq, Sk, heads, group;           // group = heads / kv_heads
-    long long ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch;
-    int left, right;                    // both clamped to kUnlimited where there is no limit
-    int sinks;
-    float scale_log2, mask_below;
-    uint32_t idesc_qk, idesc_pv;        // idesc_qk without its N field
-    unsigned int* status;
+struct TileParams : WindowParams {
+    uint32_t idesc_qk, idesc_pv;             // idesc_qk without its N field
     int n_qb, n_items;
 };
-constexpr int kUnlimited = 1 << 28;          // beyond every position (Sq, Sk <= 2^24, q_start clamped to +-2^26)
-
-// The keys that queries at positions [p_first, p_last] of a sequence can see, as runs [0, a_end) and [b_lo, b_hi).
-struct Runs {
-    int a_end, b_lo, b_hi;
-};
-__device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int p_first, int p_last) {
-    Runs r;
-    r.a_end = min(p.sinks, kv);
-    r.b_lo = max(0, p_first - p.left);
-    r.b_hi = min(kv, p_last + p.right + 1);
-    if (r.b_hi <= r.b_lo) {                  // nothing but the first tokens
-        r.b_lo = r.b_hi = 0;
-    } else if (r.b_lo <= r.a_end) {          // the runs touch
-        r.b_lo = 0;
-        r.b_hi = max(r.b_hi, r.a_end);
-        r.a_end = 0;
-    }
-    return r;
-}
-__device__ __forceinline__ int sequence_keys(const WindowParams& p, int b) {
-    if (p.kv_len == nullptr) return p.Sk;
-    return min(max(p.kv_len[b], 0), p.Sk);
-}
-__device__ __forceinline__ int first_position(const WindowParams& p, int b) {
-    if (p.q_start == nullptr) return 0;
-    return min(max(p.q_start[b], -(1 << 26)), 1 << 26);
-}
-// bits [0, n) of a word, n clamped to [0, 32]
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Roles (256 threads, two CTAs per SM; registers move from the control warpgroup to the softmax warpgroup):
@@ -107,7 +60,7 @@ struct WTile {
     int k0, end, chunks;      // first key, end of its run, 32-key chunks
 };
 
-__device__ __forceinline__ WItem load_item(const WindowParams& p, int id) {
+__device__ __forceinline__ WItem load_item(const TileParams& p, int id) {
     WItem it;
     // heads fastest: the heads of a group read the same keys and values
     it.head = id % p.heads;
@@ -135,7 +88,7 @@ __device__ __forceinline__ WTile load_tile(const WItem& it, int j) {
 template <int DT, bool MASKED>
 __global__ void __launch_bounds__(WCfg::THREADS, 2)
 window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                        const __grid_constant__ CUtensorMap tm_v, const WindowParams p) {
+                        const __grid_constant__ CUtensorMap tm_v, const TileParams p) {
     using C = WCfg;
     constexpr int NST = C::NST;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -552,11 +505,15 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     if (sms <= 0) return B200_ERR_NOT_SM100;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
 
-    WindowParams p;
+    TileParams p;
     p.mask_add = d->mask_add;
     p.kv_len = d->kv_len;
     p.q_start = d->q_start;
     p.out = d->out;
+    p.q = d->q;
+    p.k = d->k;
+    p.v = d->v;
+    p.B = static_cast<int>(d->B);
     p.Sq = static_cast<int>(d->Sq);
     p.Sk = static_cast<int>(d->Sk);
     p.heads = d->heads;
@@ -577,6 +534,8 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     p.scale_log2 = d->scale * kLog2e;
     p.mask_below = d->mask_exclude_below;
     p.status = device_status_ptr();
+
+    if (token_kernel_takes(p)) return launch_window_token(p, d->dtype, sms, stream);
 
     const long long n_qb = (d->Sq + TQ - 1) / TQ;
     const long long items = n_qb * d->heads * d->B;
