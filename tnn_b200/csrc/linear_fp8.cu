@@ -25,40 +25,48 @@ struct LinearFp8Params {
     const float* x_scale;
     const float* w_scale;
     const float* bias;
-    const void* residual;
     float* y_scale;
     int M, N;
     int num_n_tiles, num_tiles, num_k_blocks, w_blocks;   // w_blocks = ceil(N / 128)
     int x_rows;                                           // rows of x in a load box
     int out_dtype, res_dtype, epilogue;
-    long long ld_xs, ld_ys, ldr;
+    long long ld_xs, ld_ys;
     uint32_t idesc;
     unsigned int* status;
 };
 
 template <int CG, int BN, int EW>
 struct Fp8Cfg {
-    static constexpr int THREADS = 64 + 32 * EW;
+    static constexpr int THREADS = 128 + 32 * EW;        // a control warpgroup, EW / 4 epilogue warpgroups
     static constexpr int COLS = BN / (EW / 4);           // accumulator columns per epilogue warp
     static constexpr int NBUF = BN == 256 ? 2 : 4;       // TMEM buffers of BN columns
     static constexpr int TMEM_COLS = BN * NBUF;
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int B_BYTES = BN / CG * 128;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STRIP_BYTES = 32 * 128;         // one warp's output staging: 32 rows of 128 bytes
-    static constexpr int TAIL_BYTES = EW * STRIP_BYTES + 512;
+    static constexpr int STRIP_BYTES = 32 * 128;         // 32 rows of 128 bytes
+    static constexpr int STRIPS = 2;                     // per epilogue warp: output staging, before that the residual
+    static constexpr int BIAS_BYTES = EW * COLS * 4;
+    static constexpr int TAIL_BYTES = EW * STRIPS * STRIP_BYTES + BIAS_BYTES + 512;
     static constexpr int FIT = (227 * 1024 - 1024 - TAIL_BYTES) / STAGE_BYTES;
     static constexpr int STAGES = FIT > 8 ? 8 : FIT;
     static constexpr int OUT_OFFSET = STAGES * STAGE_BYTES;
-    static constexpr int BAR_OFFSET = OUT_OFFSET + EW * STRIP_BYTES;
+    static constexpr int BIAS_OFFSET = OUT_OFFSET + EW * STRIPS * STRIP_BYTES;
+    static constexpr int BAR_OFFSET = BIAS_OFFSET + BIAS_BYTES;
     static constexpr int SMEM_BYTES = OUT_OFFSET + TAIL_BYTES + 1024;
-    static_assert(STAGES >= 3 && TMEM_COLS <= 512 && COLS % 32 == 0, "tile does not fit");
+    // 128 sums per thread and 32 values in flight do not fit the 168 registers that 384 threads get at launch (with them
+    // spilled, a k-block's promotion took 0.9 us instead of 0.4): the control warpgroup hands most of its own over.
+    static constexpr bool MOVE_REGS = EW == 8 && COLS == 128;
+    static constexpr int REGS_CONTROL = 40, REGS_EPILOGUE = 232;
+    static_assert(!MOVE_REGS || 128 * REGS_CONTROL + 256 * REGS_EPILOGUE <= THREADS * (65536 / THREADS / 8 * 8),
+                  "setmaxnreg: the epilogue's registers must come out of the CTA's own pool");
+    static_assert(STAGES >= 3 && TMEM_COLS <= 512 && COLS % 64 == 0, "tile does not fit");
 };
 
 template <int CG, int BN, int EW, int OUT>
-__global__ void __launch_bounds__(64 + 32 * EW, 1)
+__global__ void __launch_bounds__(128 + 32 * EW, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                  const __grid_constant__ CUtensorMap tm_y, const LinearFp8Params p) {
+                  const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_r, const LinearFp8Params p) {
     using C = Fp8Cfg<CG, BN, EW>;
     constexpr int STAGES = C::STAGES, NBUF = C::NBUF, COLS = C::COLS;
     extern __shared__ uint8_t smem_raw[];
@@ -68,7 +76,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + NBUF;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + NBUF);
+    uint64_t* res_full = acc_empty + NBUF;              // [EW]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + EW);
     volatile uint32_t* abort_flag = tmem_slot + 1;
 
     const int warp = threadIdx.x >> 5;
@@ -87,6 +96,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], CG * EW);   // leader's copy: epilogue warps of all its CTAs
         }
+        for (int w = 0; w < EW; ++w) mbar_init(&res_full[w], 1);
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tm_x);
@@ -115,9 +125,10 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     }
     pdl_wait();
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer (every CTA its own part)
-        if (elect_one()) {
+    if (warp < 4) {
+        if (C::MOVE_REGS) setmaxnreg_dec<C::REGS_CONTROL>();
+        if (warp == 0 && elect_one()) {
+            // -------------------------------------------------------- TMA producer (every CTA its own part)
             uint32_t st = 0, ph = 0;
             bool ok = true;
             const uint32_t bytes = CG * (static_cast<uint32_t>(p.x_rows) * 128 + C::B_BYTES);
@@ -145,10 +156,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                 for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
             }
         }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ UMMA issuer (leader CTA only)
-        if (leader && elect_one()) {
+        if (warp == 1 && leader && elect_one()) {
+            // -------------------------------------------------------- UMMA issuer (leader CTA only)
             uint32_t st = 0, ph = 0, buf = 0, bph = 0;
             bool ok = true;
             const uint64_t a_desc0 = make_smem_desc_sw128(smem_u32(smem));
@@ -177,41 +186,78 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         }
         __syncwarp();
     } else {
+        if (C::MOVE_REGS) setmaxnreg_inc<C::REGS_EPILOGUE>();
         // ------------------------------------------------------------ scale, add, store (own 128 rows)
-        const int ew = warp - 2;
+        const int ew = warp - 4;
         const int quarter = warp & 3;
         const int col_first = (ew >> 2) * COLS;
-        uint8_t* strip = smem + C::OUT_OFFSET + ew * C::STRIP_BYTES;
-        uint8_t* srow = strip + lane * 128;
+        uint8_t* strips = smem + C::OUT_OFFSET + ew * C::STRIPS * C::STRIP_BYTES;
         const int sw = lane & 7;            // 128-byte swizzle: 16-byte piece i of row r lies at i ^ (r & 7)
+        float* bias_s = reinterpret_cast<float*>(smem + C::BIAS_OFFSET) + ew * COLS;
         const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_first;
-        uint32_t buf = 0, bph = 0;
+        const bool res = p.epilogue == B200_EPI_BIAS_RESIDUAL;
+        uint32_t buf = 0, bph = 0, rph = 0;
         bool ok = true;
+        // The scales of this thread's row and of the warp's columns, fetched two k-blocks ahead, over the end of a tile too:
+        // their way from L2 is longer than a k-block (fetched one ahead, 16384 x 4096 x 4096 on 128-wide tiles took 556 us, so 373).
+        struct Ahead {
+            int tile, kb;
+            const float *xs, *ws;
+        } at = {group - num_groups, 0, nullptr, nullptr};
+        auto next_tile = [&]() {
+            at.tile += num_groups;
+            at.kb = 0;
+            const int r = at.tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+            const int b = (at.tile % p.num_n_tiles * BN + col_first) / fp8::kBlock;
+            at.xs = p.x_scale + (r < p.M ? r : 0);
+            at.ws = p.w_scale + static_cast<long long>(b < p.w_blocks ? b : p.w_blocks - 1) * p.num_k_blocks;
+        };
+        auto fetch_scales = [&](float& x, float& w) {
+            if (at.tile >= p.num_tiles) return;
+            x = __ldg(at.xs);
+            w = __ldg(at.ws);
+            at.xs += p.ld_xs;
+            ++at.ws;
+            if (++at.kb == p.num_k_blocks) next_tile();
+        };
+        float x_s[2] = {0.f, 0.f}, w_s[2] = {0.f, 0.f};
+        next_tile();
+        fetch_scales(x_s[0], w_s[0]);
+        fetch_scales(x_s[1], w_s[1]);
         for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
             const int row0 = tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128 + quarter * 32;
-            const int row = row0 + lane;
             const int n_first = tile % p.num_n_tiles * BN + col_first;
-            const bool row_ok = row < p.M;
-            // the scale of this thread's row and of the warp's columns, one k-block ahead
-            const float* xs = p.x_scale + (row_ok ? row : 0);
-            const int wb = n_first / fp8::kBlock;
-            const float* ws = p.w_scale + static_cast<long long>(wb < p.w_blocks ? wb : p.w_blocks - 1) * p.num_k_blocks;
-            float s_next = __ldg(xs) * __ldg(ws);
+            // what this warp stores of the tile: 64-column pieces of its 32 rows (the store clips what lies outside y)
+            const int pieces = row0 < p.M && n_first < p.N ? min(COLS / 64, (p.N - n_first + 63) / 64) : 0;
+            __syncwarp();   // every lane has read the previous tile's bias
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < COLS / 32; ++i) {
+                    const int n = n_first + i * 32 + lane;
+                    bias_s[i * 32 + lane] = n < p.N ? __ldg(p.bias + n) : 0.f;
+                }
+            }
             uint64_t acc[COLS / 2];
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
             for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-                const uint64_t s2 = pack_f32x2(s_next, s_next);
-                if (kb + 1 < p.num_k_blocks) s_next = __ldg(xs + (kb + 1) * p.ld_xs) * __ldg(ws + kb + 1);
+                const float scale = x_s[0] * w_s[0];
+                const uint64_t s2 = pack_f32x2(scale, scale);
+                x_s[0] = x_s[1];
+                w_s[0] = w_s[1];
+                fetch_scales(x_s[1], w_s[1]);
                 if (!mbar_wait(&acc_full[buf], bph, abort_flag)) { ok = false; break; }
                 __syncwarp();
                 tcgen05_fence_after();
+                // 32 columns travel while the 32 before them are added
+                uint32_t r[2][32];
+                tmem_ld_32x32b_x32(tacc + buf * BN, r[0]);
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(tacc + buf * BN + c * 32, r);
-                    tmem_ld_wait(r);
-                    if (c == COLS / 32 - 1) {   // the buffer is in registers: hand it back
+                    tmem_ld_wait(r[c & 1]);
+                    if (c + 1 < COLS / 32) {
+                        tmem_ld_32x32b_x32(tacc + buf * BN + (c + 1) * 32, r[(c + 1) & 1]);
+                    } else {   // the buffer is in registers: hand it back
                         tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -221,31 +267,38 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        acc[c * 16 + j] = fma_f32x2(pack_f32x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2,
+                        acc[c * 16 + j] = fma_f32x2(pack_f32x2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), s2,
                                                     acc[c * 16 + j]);
                 }
                 if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+                if (kb == 0 && res && pieces > 0 && lane == 0) {
+                    // the residual of this tile into the strips, which the previous tile's stores have read by now
+                    tma_store_wait_read<0>();
+                    mbar_expect_tx(&res_full[ew], static_cast<uint32_t>(pieces) * C::STRIP_BYTES);
+                    for (int i = 0; i < pieces; ++i)
+                        tma_load_2d(strips + i * C::STRIP_BYTES, &tm_r, &res_full[ew], n_first + i * 64, row0);
+                }
             }
             if (!ok) break;
+            if (pieces == 0) continue;
+            if (res) {
+                if (!mbar_wait(&res_full[ew], rph, abort_flag)) { ok = false; break; }
+                rph ^= 1u;
+                __syncwarp();
+            }
 
-            // bias, activation, residual
+            // bias, activation, residual: 32 columns in place
             uint32_t bits = 0;
-#pragma unroll
-            for (int c = 0; c < COLS / 32; ++c) {
-                const int n0 = n_first + c * 32;
-                float v[32];
+            auto finish = [&](int c, float (&v)[32]) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1]);
                 if (p.bias != nullptr) {
 #pragma unroll
-                    for (int g = 0; g < 8; ++g)
-                        if (n0 + g * 4 < p.N) {
-                            const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0) + g);
-                            v[g * 4 + 0] += b.x;
-                            v[g * 4 + 1] += b.y;
-                            v[g * 4 + 2] += b.z;
-                            v[g * 4 + 3] += b.w;
-                        }
+                    for (int g = 0; g < 8; ++g) {
+                        const float4 b = *reinterpret_cast<const float4*>(bias_s + c * 32 + g * 4);
+                        unpack_f32x2(add_f32x2(pack_f32x2(v[g * 4 + 0], v[g * 4 + 1]), pack_f32x2(b.x, b.y)), v[g * 4 + 0], v[g * 4 + 1]);
+                        unpack_f32x2(add_f32x2(pack_f32x2(v[g * 4 + 2], v[g * 4 + 3]), pack_f32x2(b.z, b.w)), v[g * 4 + 2], v[g * 4 + 3]);
+                    }
                 }
                 if (p.epilogue == B200_EPI_BIAS_GELU) {
                     if (OUT == kOutF32) {   // nothing rounds the result: the library's erf
@@ -261,83 +314,117 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         if (OUT == kOutF32) v[j] = tanhf(v[j]);
                         else asm("tanh.approx.f32 %0, %1;" : "=f"(v[j]) : "f"(v[j]));
                     }
-                } else if (p.epilogue == B200_EPI_BIAS_RESIDUAL && row_ok) {
-                    const uint16_t* rp = static_cast<const uint16_t*>(p.residual) + row * p.ldr + n0;
+                } else if (res && c / 2 < pieces) {
+                    const uint8_t* srow = strips + (c / 2) * C::STRIP_BYTES + lane * 128;
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        if (n0 + g * 8 < p.N) {
-                            const uint4 q = __ldg(reinterpret_cast<const uint4*>(rp + g * 8));
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                    for (int g = 0; g < 4; ++g) {
+                        const uint4 q = *reinterpret_cast<const uint4*>(srow + ((((c & 1) * 4 + g) ^ sw) << 4));
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 f = unpack2(w[e], p.res_dtype);
-                                v[g * 8 + 2 * e] += f.x;
-                                v[g * 8 + 2 * e + 1] += f.y;
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = unpack2(w[e], p.res_dtype);
+                            v[g * 8 + 2 * e] += f.x;
+                            v[g * 8 + 2 * e + 1] += f.y;
                         }
+                    }
                 }
-                if (OUT == kOutF8) {
-                    // columns at or beyond N are zeros (no weight, no bias, no residual): they do not move the maximum
+            };
+            if (OUT == kOutHalf) {
+                // a strip holds 64 columns; with a residual a thread replaces its own row's values in it
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) bits = max(bits, fp8::abs_bits(v[j]));
+                for (int h = 0; h < COLS / 64; ++h) {
+                    if (h >= pieces) break;
+                    uint8_t* srow = strips + h * C::STRIP_BYTES + lane * 128;
+                    if (!res) {   // the strip's store of the previous tile has read it
+                        if (lane == 0) tma_store_wait_read<COLS / 64 - 1>();
+                        __syncwarp();
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c * 16 + j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
-                    continue;
+                    for (int cc = 0; cc < 2; ++cc) {
+                        float v[32];
+                        finish(h * 2 + cc, v);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            uint4 q;
+                            q.x = pack2(v[g * 8 + 0], v[g * 8 + 1], p.out_dtype);
+                            q.y = pack2(v[g * 8 + 2], v[g * 8 + 3], p.out_dtype);
+                            q.z = pack2(v[g * 8 + 4], v[g * 8 + 5], p.out_dtype);
+                            q.w = pack2(v[g * 8 + 6], v[g * 8 + 7], p.out_dtype);
+                            *reinterpret_cast<uint4*>(srow + (((cc * 4 + g) ^ sw) << 4)) = q;
+                        }
+                    }
+                    fence_async_proxy_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tm_y, strips + h * C::STRIP_BYTES, n_first + h * 64, row0);
+                        tma_store_commit();
+                    }
                 }
-                constexpr int PER_STRIP = OUT == kOutF32 ? 1 : 2;   // 32-column chunks in a strip
-                if (c % PER_STRIP == 0) {
-                    if (lane == 0) tma_store_wait_read<0>();   // the strip's previous store has read it
+            } else {
+                if (OUT == kOutF8 || res) {   // everything but the store first: the strips' residual makes way for the output
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        float v[32];
+                        finish(c, v);
+                        if (OUT == kOutF8) {
+                            // columns at or beyond N are zeros (no weight, no bias, no residual): they do not move the maximum
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) bits = max(bits, fp8::abs_bits(v[j]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[c * 16 + j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
+                    }
                     __syncwarp();
                 }
                 if (OUT == kOutF32) {
 #pragma unroll
-                    for (int g = 0; g < 8; ++g)
-                        *reinterpret_cast<float4*>(srow + ((g ^ sw) << 4)) =
-                            make_float4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
-                } else {
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        if (n_first + c * 32 >= p.N) break;
+                        uint8_t* srow = strips + (c & 1) * C::STRIP_BYTES + lane * 128;
+                        float v[32];
+                        if (res) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        uint4 q;
-                        q.x = pack2(v[g * 8 + 0], v[g * 8 + 1], p.out_dtype);
-                        q.y = pack2(v[g * 8 + 2], v[g * 8 + 3], p.out_dtype);
-                        q.z = pack2(v[g * 8 + 4], v[g * 8 + 5], p.out_dtype);
-                        q.w = pack2(v[g * 8 + 6], v[g * 8 + 7], p.out_dtype);
-                        *reinterpret_cast<uint4*>(srow + ((((c & 1) * 4 + g) ^ sw) << 4)) = q;
+                            for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1]);
+                        } else {
+                            finish(c, v);
+                        }
+                        if (lane == 0) tma_store_wait_read<1>();   // the strip's last store has read it
+                        __syncwarp();
+#pragma unroll
+                        for (int g = 0; g < 8; ++g)
+                            *reinterpret_cast<float4*>(srow + ((g ^ sw) << 4)) = make_float4(v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]);
+                        fence_async_proxy_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tm_y, strips + (c & 1) * C::STRIP_BYTES, 2 * (n_first + c * 32), row0);
+                            tma_store_commit();
+                        }
                     }
-                }
-                if (c % PER_STRIP == PER_STRIP - 1) {
+                } else {
+                    const float amax = fp8::amax_of_bits(bits);
+                    const float enc = fp8::encode_scale(amax);
+                    uint8_t* srow = strips + lane * 128;
+                    if (lane == 0) tma_store_wait_read<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int g = 0; g < COLS / 16; ++g) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float a0, a1, a2, a3;
+                            unpack_f32x2(acc[g * 8 + e * 2], a0, a1);
+                            unpack_f32x2(acc[g * 8 + e * 2 + 1], a2, a3);
+                            w[e] = fp8::pack4(a0 * enc, a1 * enc, a2 * enc, a3 * enc);
+                        }
+                        *reinterpret_cast<uint4*>(srow + ((g ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    if (row0 + lane < p.M) p.y_scale[n_first / fp8::kBlock * p.ld_ys + row0 + lane] = fp8::decode_scale(amax);
                     fence_async_proxy_shared();
                     __syncwarp();
-                    const int n_strip = n_first + (c / PER_STRIP) * PER_STRIP * 32;
-                    if (lane == 0 && n_strip < p.N && row0 < p.M) {   // the store clips rows and columns outside y
-                        tma_store_2d(&tm_y, strip, OUT == kOutF32 ? 2 * n_strip : n_strip, row0);
+                    if (lane == 0) {
+                        tma_store_2d(&tm_y, strips, n_first / 2, row0);
                         tma_store_commit();
                     }
-                }
-            }
-            if (OUT == kOutF8) {
-                const float amax = fp8::amax_of_bits(bits);
-                const float enc = fp8::encode_scale(amax);
-                if (lane == 0) tma_store_wait_read<0>();
-                __syncwarp();
-#pragma unroll
-                for (int g = 0; g < COLS / 16; ++g) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float a0, a1, a2, a3;
-                        unpack_f32x2(acc[g * 8 + e * 2], a0, a1);
-                        unpack_f32x2(acc[g * 8 + e * 2 + 1], a2, a3);
-                        w[e] = fp8::pack4(a0 * enc, a1 * enc, a2 * enc, a3 * enc);
-                    }
-                    *reinterpret_cast<uint4*>(srow + ((g ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                if (row_ok && n_first < p.N) p.y_scale[wb * p.ld_ys + row] = fp8::decode_scale(amax);
-                fence_async_proxy_shared();
-                __syncwarp();
-                if (lane == 0 && n_first < p.N && row0 < p.M) {
-                    tma_store_2d(&tm_y, strip, n_first / 2, row0);
-                    tma_store_commit();
                 }
             }
         }
@@ -428,7 +515,7 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
     if (groups <= 0) return B200_ERR_LAUNCH;
     // Rows that do not exist are not fetched where all rows fit one box: what the stage holds there feeds no stored row.
     const int x_rows = CG == 1 && d.M < 128 ? static_cast<int>((d.M + 7) / 8 * 8) : 128;
-    CUtensorMap tx, tw, ty;
+    CUtensorMap tx, tw, ty, tr;
     {   // two e4m3 values as one 16-bit element
         const uint64_t xd[2] = {static_cast<uint64_t>(d.K / 2), static_cast<uint64_t>(d.M)};
         const uint64_t xs[1] = {static_cast<uint64_t>(d.ldx)};
@@ -443,12 +530,15 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
         if (!get_tensor_map(&tx, d.x, 2, xd, xs, xb) || !get_tensor_map(&tw, d.w_nk, 2, wd, ws, wb) ||
             !get_tensor_map(&ty, d.y, 2, yd, ys, yb))
             return B200_ERR_DRIVER;
+        tr = ty;   // unused without a residual
+        const uint64_t rd[2] = {static_cast<uint64_t>(d.N), static_cast<uint64_t>(d.M)};
+        const uint64_t rs[1] = {static_cast<uint64_t>(d.ldr) * 2};
+        if (d.epilogue == B200_EPI_BIAS_RESIDUAL && !get_tensor_map(&tr, d.residual, 2, rd, rs, yb)) return B200_ERR_DRIVER;
     }
     LinearFp8Params p;
     p.x_scale = d.x_scale;
     p.w_scale = d.w_scale;
     p.bias = d.bias;
-    p.residual = d.residual;
     p.y_scale = d.y_scale;
     p.M = static_cast<int>(d.M);
     p.N = static_cast<int>(d.N);
@@ -464,12 +554,11 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
     p.epilogue = d.epilogue;
     p.ld_xs = d.ld_x_scale;
     p.ld_ys = d.ld_y_scale;
-    p.ldr = d.ldr;
     p.idesc = make_idesc_f16(128 * CG, BN, 0, 0, 0);   // format code 0 of kind::f8f6f4 = e4m3
     p.status = device_status_ptr();
     const int used = p.num_tiles < groups ? p.num_tiles : groups;
     launch_groups<CG>(linear_fp8_kernel<CG, BN, EW, OUT>, static_cast<unsigned>(used * CG), C::THREADS, C::SMEM_BYTES, stream, tx, tw,
-                      ty, p);
+                      ty, tr, p);
     count_launch();
     return check_launch();
 }
