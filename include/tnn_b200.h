@@ -342,7 +342,7 @@ B200_API int b200_add_layernorm_fp8_fwd(const B200LayerNormFp8Desc* desc, b200_s
  *   GELU and tanh use the fast forms of b200_linear_fwd (absolute deviation 3e-5, relative 2^-11) unless y is F32.
  *   Requirements: K % 16 == 0, N % 8 == 0 (16 for E4M3), ldx, ldw % 16 == 0, ldy % 8 == 0 (16), ldr % 8 == 0, K <= 2^24,
  *   ld_x_scale and ld_y_scale >= M, 16-byte aligned pointers (scales: 4-byte).
- *   block_n: 0 = choose the tile; 128, 256: CTA-pair tiles (256 x block_n); -64 (not for E4M3), -128: single-CTA tiles. */
+ *   block_n: 0 = choose the tile; 64 (not for E4M3), 128, 256: tiles of 128 x block_n, for testing. */
 typedef struct B200LinearFp8Desc {
     const void*  x;
     const void*  w_nk;

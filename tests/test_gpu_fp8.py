@@ -174,7 +174,7 @@ def test_linear_fp8(cuda_device, M, N, K, out):
     assert torch.equal(y, ops.linear_fp8(x8, xs, w8, ws, bias, out_dtype=out))
 
 
-@pytest.mark.parametrize("block_n", [-64, -128, 128, 256])
+@pytest.mark.parametrize("block_n", [64, 128, 256])
 @pytest.mark.parametrize("epi", ["none", "bias", "gelu", "tanh", "residual"])
 @pytest.mark.parametrize("M,N,K", [(41, 200, 400), (300, 392, 272), (513, 256, 128)])
 def test_linear_fp8_epilogues_on_every_tile(cuda_device, M, N, K, epi, block_n):
@@ -204,7 +204,7 @@ def test_linear_fp8_epilogues_on_every_tile(cuda_device, M, N, K, epi, block_n):
         assert bool((err <= bound).all()), float((err - bound).max())
 
 
-@pytest.mark.parametrize("block_n", [0, -128, 128, 256])
+@pytest.mark.parametrize("block_n", [0, 128, 256])
 @pytest.mark.parametrize("epi", ["bias", "gelu", "residual"])
 @pytest.mark.parametrize("M,N,K", [(1, 16, 64), (41, 272, 400), (300, 1040, 256), (129, 128, 144)])
 def test_linear_fp8_with_an_8_bit_result(cuda_device, M, N, K, epi, block_n):
@@ -235,12 +235,12 @@ def test_linear_fp8_rows_do_not_depend_on_the_batch_or_the_tile(cuda_device):
     for rows in (slice(0, 1), slice(3, 44), slice(100, 400)):
         part = ops.linear_fp8(x8[rows], xs[:, rows].contiguous(), w8, ws, bias, out_dtype=F32)
         assert torch.equal(part, y[rows])
-    for bn in (-64, -128, 128, 256):
+    for bn in (64, 128, 256):
         assert torch.equal(ops.linear_fp8(x8, xs, w8, ws, bias, out_dtype=F32, block_n=bn), y)
 
 
 @pytest.mark.parametrize("out", [F16, F32, F8])
-@pytest.mark.parametrize("M,N,block_n", [(1, 80, 0), (41, 272, -128), (300, 272, 256), (130, 144, 128)])
+@pytest.mark.parametrize("M,N,block_n", [(1, 80, 0), (41, 272, 128), (300, 272, 256), (130, 144, 128)])
 def test_linear_fp8_strides_and_what_lies_around_the_output(cuda_device, M, N, block_n, out):
     K = 272
     x8, xs, w8, ws = _operands(cuda_device, M, N, K, 3)

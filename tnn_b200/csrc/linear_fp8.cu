@@ -1,18 +1,19 @@
 // Projection / FFN GEMM on 8-bit operands with block scales:
 //   y[m, n] = epilogue(sum_b xs[b, m] * ws[n / 128, b] * sum_{k in block b} x8[m, k] w8[n, k] + bias[n] (+ r[m, n])).
 //
-// The scales change every 128 values of K, so the tensor cores may not add across blocks.  A k-block of a pipeline stage is
+// The scales change every 128 values of K, so the tensor core may not add across blocks.  A k-block of a pipeline stage is
 // exactly one scale block (128 e4m3 values = one 128-byte swizzled row): its four UMMAs (kind::f8f6f4, K = 32 each) start a
-// fresh accumulator in one of NBUF TMEM buffers, and the epilogue warps add scale * buffer to fp32 sums that stay in their
-// registers for the whole tile (thread = row, COLS columns), while the tensor pipe fills the other buffers.  Products are
-// exact in fp32; the sum inside a block is the tensor core's fp32 accumulation, the sum over blocks one fp32 FMA each, in
-// ascending order whatever the tile, so a row's result depends on neither the batch nor the tile chosen.
+// fresh accumulator in a TMEM buffer, and the epilogue warps add scale * buffer to fp32 sums that stay in their registers for
+// the whole tile (thread = row, COLS columns), while the tensor pipe fills the other buffers.  Products are exact in fp32; the
+// sum inside a block is the tensor core's fp32 accumulation, the sum over blocks one fp32 FMA each, in ascending order whatever
+// the tile, so a row's result depends on neither the batch nor the tile chosen.
 //
-// CG = 2: pairs of SMs (cta_group::2) on a 256 x BN tile, each CTA loading its 128 rows of x and BN / 2 rows of w;
-// CG = 1: one SM on 128 x BN, for launches of few rows.  Roles as in linear_pair.cu: warp 0 TMA producer, warp 1 TMEM
-// allocation and UMMA issue (in the leader CTA), the other EW warps scale, add and store.
+// A tile is 128 x BN on one SM.
+//   warp 0      : TMA producer
+//   warp 1      : TMEM allocation, UMMA issue (one elected lane)
+//   warps 4 ..  : EW epilogue warps: scale and add, then bias / activation / residual and the store
 #include "fp8.cuh"
-#include "pair.cuh"
+#include "linear_common.cuh"
 
 namespace b200 {
 namespace lin {
@@ -35,42 +36,44 @@ struct LinearFp8Params {
     unsigned int* status;
 };
 
-template <int CG, int BN, int EW>
+template <int BN, int EW>
 struct Fp8Cfg {
     static constexpr int THREADS = 128 + 32 * EW;        // a control warpgroup, EW / 4 epilogue warpgroups
     static constexpr int COLS = BN / (EW / 4);           // accumulator columns per epilogue warp
     static constexpr int NBUF = BN == 256 ? 2 : 4;       // TMEM buffers of BN columns
     static constexpr int TMEM_COLS = BN * NBUF;
     static constexpr int A_BYTES = 128 * 128;
-    static constexpr int B_BYTES = BN / CG * 128;
+    static constexpr int B_BYTES = BN * 128;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STRIP_BYTES = 32 * 128;         // 32 rows of 128 bytes
     static constexpr int STRIPS = 2;                     // per epilogue warp: output staging, before that the residual
     static constexpr int BIAS_BYTES = EW * COLS * 4;
-    static constexpr int TAIL_BYTES = EW * STRIPS * STRIP_BYTES + BIAS_BYTES + 512;
+    static constexpr int GROUPS = BN == 256 ? 2 : 1;     // 128-column scale blocks of a tile, a scale warp each
+    static constexpr int SCALE_BYTES = GROUPS * NBUF * 128 * 4;   // one per row, group and TMEM buffer
+    static constexpr int TAIL_BYTES = EW * STRIPS * STRIP_BYTES + BIAS_BYTES + SCALE_BYTES + 512;
     static constexpr int FIT = (227 * 1024 - 1024 - TAIL_BYTES) / STAGE_BYTES;
     static constexpr int STAGES = FIT > 8 ? 8 : FIT;
     static constexpr int OUT_OFFSET = STAGES * STAGE_BYTES;
     static constexpr int BIAS_OFFSET = OUT_OFFSET + EW * STRIPS * STRIP_BYTES;
-    static constexpr int BAR_OFFSET = BIAS_OFFSET + BIAS_BYTES;
+    static constexpr int SCALE_OFFSET = BIAS_OFFSET + BIAS_BYTES;
+    static constexpr int BAR_OFFSET = SCALE_OFFSET + SCALE_BYTES;
     static constexpr int SMEM_BYTES = OUT_OFFSET + TAIL_BYTES + 1024;
     // 128 sums per thread and 32 values in flight do not fit the 168 registers that 384 threads get at launch (with them
     // spilled, a k-block's promotion took 0.9 us instead of 0.4): the control warpgroup hands most of its own over.
     static constexpr bool MOVE_REGS = EW == 8 && COLS == 128;
-    static constexpr int REGS_CONTROL = 40, REGS_EPILOGUE = 232;
+    static constexpr int REGS_CONTROL = 56, REGS_EPILOGUE = 224;
     static_assert(!MOVE_REGS || 128 * REGS_CONTROL + 256 * REGS_EPILOGUE <= THREADS * (65536 / THREADS / 8 * 8),
                   "setmaxnreg: the epilogue's registers must come out of the CTA's own pool");
     static_assert(STAGES >= 3 && TMEM_COLS <= 512 && COLS % 64 == 0, "tile does not fit");
 };
 
-template <int CG, int BN, int EW, int OUT>
+template <int BN, int EW, int OUT>
 __global__ void __launch_bounds__(128 + 32 * EW, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_r, const LinearFp8Params p) {
-    using C = Fp8Cfg<CG, BN, EW>;
+    using C = Fp8Cfg<BN, EW>;
     constexpr int STAGES = C::STAGES, NBUF = C::NBUF, COLS = C::COLS;
     extern __shared__ uint8_t smem_raw[];
-    // Rounding up gives the same offset in both CTAs of a pair: the dynamic window starts at the same place in each.
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFFSET);
     uint64_t* empty = full + STAGES;
@@ -79,22 +82,18 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     uint64_t* res_full = acc_empty + NBUF;              // [EW]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + EW);
     volatile uint32_t* abort_flag = tmem_slot + 1;
+    float* scale_s = reinterpret_cast<float*>(smem + C::SCALE_OFFSET);   // [NBUF][GROUPS][128]
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
-    const bool leader = rank == 0;
-    const int group = blockIdx.x / CG;
-    const int num_groups = gridDim.x / CG;
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], 1);    // the leader's expect_tx arrival
-            mbar_init(&empty[s], 1);   // one commit per use
+            mbar_init(&full[s], 1);    // the producer's expect_tx arrival
+            mbar_init(&empty[s], 1);   // an epilogue warp, once the stage's UMMAs are done
         }
         for (int b = 0; b < NBUF; ++b) {
-            mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], CG * EW);   // leader's copy: epilogue warps of all its CTAs
+            mbar_init(&acc_full[b], 1 + C::GROUPS);   // the UMMAs' commit and the scale warps
+            mbar_init(&acc_empty[b], EW);
         }
         for (int w = 0; w < EW; ++w) mbar_init(&res_full[w], 1);
         *abort_flag = 0;
@@ -103,84 +102,122 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         prefetch_tmap(&tm_w);
     }
     if (warp == 1) {
-        if (CG == 2) {
-            tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
-            tmem_relinquish_pair();
-        } else {
-            tmem_alloc(tmem_slot, C::TMEM_COLS);
-            tmem_relinquish();
-        }
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync_all();   // the peer's barriers and TMEM are set up before anything is signalled
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         // The weights' way from HBM to L2 starts while the previous kernel of the stream drains (a hint, no data is taken).
-        const int row_boxes = (p.N + BN / CG - 1) / (BN / CG);
-        for (int b = blockIdx.x; b < p.num_k_blocks * row_boxes; b += gridDim.x)
-            tma_prefetch_l2_2d(&tm_w, (b % p.num_k_blocks) * 64, (b / p.num_k_blocks) * (BN / CG));
+        for (int b = blockIdx.x; b < p.num_k_blocks * p.num_n_tiles; b += gridDim.x)
+            tma_prefetch_l2_2d(&tm_w, (b % p.num_k_blocks) * 64, (b / p.num_k_blocks) * BN);
     }
     pdl_wait();
 
     if (warp < 4) {
         if (C::MOVE_REGS) setmaxnreg_dec<C::REGS_CONTROL>();
-        if (warp == 0 && elect_one()) {
-            // -------------------------------------------------------- TMA producer (every CTA its own part)
-            uint32_t st = 0, ph = 0;
-            bool ok = true;
-            const uint32_t bytes = CG * (static_cast<uint32_t>(p.x_rows) * 128 + C::B_BYTES);
-            for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
-                const int x_row = tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128;
-                const int w_row = tile % p.num_n_tiles * BN + static_cast<int>(rank) * (BN / CG);
-                for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-                    if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    uint8_t* a = smem + st * C::STAGE_BYTES;
-                    uint8_t* b = a + C::A_BYTES;
-                    if (leader) mbar_expect_tx(&full[st], bytes);
-                    // the maps count 16-bit units: a k-block is 64 of them
-                    if (CG == 2) {
-                        const uint32_t bar = leader_addr(&full[st]);
-                        tma_load_2d_pair(a, &tm_x, bar, kb * 64, x_row);
-                        tma_load_2d_pair(b, &tm_w, bar, kb * 64, w_row);
-                    } else {
+        if (warp == 0) {
+            // -------------------------------------------------------- TMA producer
+            if (elect_one()) {
+                uint32_t st = 0, ph = 0;
+                bool ok = true;
+                const uint32_t bytes = static_cast<uint32_t>(p.x_rows) * 128 + C::B_BYTES;
+                for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+                    const int x_row = tile / p.num_n_tiles * 128, w_row = tile % p.num_n_tiles * BN;
+                    for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+                        if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag)) { ok = false; break; }
+                        uint8_t* a = smem + st * C::STAGE_BYTES;
+                        mbar_expect_tx(&full[st], bytes);
+                        // the maps count 16-bit units: a k-block is 64 of them
                         tma_load_2d(a, &tm_x, &full[st], kb * 64, x_row);
-                        tma_load_2d(b, &tm_w, &full[st], kb * 64, w_row);
+                        tma_load_2d(a + C::A_BYTES, &tm_w, &full[st], kb * 64, w_row);
+                        if (++st == STAGES) { st = 0; ph ^= 1u; }
                     }
-                    if (++st == STAGES) { st = 0; ph ^= 1u; }
+                }
+                if (!ok) {
+                    for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
                 }
             }
-            if (!ok) {
-                for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
-            }
-        }
-        if (warp == 1 && leader && elect_one()) {
-            // -------------------------------------------------------- UMMA issuer (leader CTA only)
-            uint32_t st = 0, ph = 0, buf = 0, bph = 0;
-            bool ok = true;
-            const uint64_t a_desc0 = make_smem_desc_sw128(smem_u32(smem));
-            const uint64_t b_desc0 = make_smem_desc_sw128(smem_u32(smem + C::A_BYTES));
-            for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
-                for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-                    if (!mbar_wait(&acc_empty[buf], bph ^ 1u, abort_flag) || !mbar_wait(&full[st], ph, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    tcgen05_fence_after();
-                    const uint32_t d_tmem = tmem_base + buf * BN;
-                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
-                    const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
+        } else if (warp == 1) {
+            // -------------------------------------------------------- UMMA issuer
+            if (elect_one()) {
+                uint32_t st = 0, ph = 0, buf = 0, bph = 0;
+                bool ok = true;
+                const uint64_t a_desc0 = make_smem_desc_sw128(smem_u32(smem));
+                const uint64_t b_desc0 = make_smem_desc_sw128(smem_u32(smem + C::A_BYTES));
+                for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+                    for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+                        if (!mbar_wait(&full[st], ph, abort_flag) || !mbar_wait(&acc_empty[buf], bph ^ 1u, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tcgen05_fence_after();
+                        const uint32_t d_tmem = tmem_base + buf * BN;
+                        const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
+                        const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(st * (C::STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (CG == 2) umma_f8_ss_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, p.idesc, k != 0 ? 1u : 0u);
-                        else umma_f8_ss(d_tmem, a_desc + 2 * k, b_desc + 2 * k, p.idesc, k != 0 ? 1u : 0u);
+                        for (int k = 0; k < 4; ++k) umma_f8_ss(d_tmem, a_desc + 2 * k, b_desc + 2 * k, p.idesc, k != 0 ? 1u : 0u);
+                        // One commit a k-block (each costs the tensor pipe 30 to 60 clocks): the epilogue hands the stage back.
+                        umma_f8_commit(&acc_full[buf]);
+                        if (++st == STAGES) { st = 0; ph ^= 1u; }
+                        if (++buf == NBUF) { buf = 0; bph ^= 1u; }
                     }
-                    umma_f8_commit(&empty[st], CG == 2);
-                    umma_f8_commit(&acc_full[buf], CG == 2);
-                    if (++st == STAGES) { st = 0; ph ^= 1u; }
-                    if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+                }
+            }
+        } else if (warp - 2 < C::GROUPS) {
+            // -------------------------------------------------------- scales: x_scale * w_scale of the rows and a column group
+            // Loads U k-blocks ahead, over the end of a tile too: their way from L2 is longer than a k-block.  Slot u holds
+            // k-blocks u, u + U, ... of a tile, then u of the next one.
+            constexpr int U = 2;
+            const int g = warp - 2;
+            float x[U][4], w[U];
+            const float *xs = nullptr, *ws = nullptr, *xs_next = nullptr, *ws_next = nullptr;
+            int there = 0, there_next = 0;   // how many of this lane's four rows exist
+            auto locate = [&](int tile) {
+                const int r = tile / p.num_n_tiles * 128 + lane;
+                const int b = (tile % p.num_n_tiles * BN + g * 128) / fp8::kBlock;
+                xs_next = p.x_scale + r;
+                ws_next = p.w_scale + static_cast<long long>(b < p.w_blocks ? b : p.w_blocks - 1) * p.num_k_blocks;
+                there_next = (p.M - r + 31) >> 5;
+            };
+            auto fetch = [&](const float* px, const float* pw, int in, int kb, float (&xv)[4], float& wv) {
+                wv = __ldg(pw + kb);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < in) xv[i] = __ldg(px + kb * p.ld_xs + 32 * i);
+            };
+            uint32_t buf = 0, bph = 0;
+            bool ok = true;
+            if (static_cast<int>(blockIdx.x) < p.num_tiles) locate(blockIdx.x);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                w[u] = x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
+                if (static_cast<int>(blockIdx.x) < p.num_tiles && u < p.num_k_blocks) fetch(xs_next, ws_next, there_next, u, x[u], w[u]);
+            }
+            for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+                xs = xs_next;
+                ws = ws_next;
+                there = there_next;
+                const bool more = tile + static_cast<int>(gridDim.x) < p.num_tiles;
+                if (more) locate(tile + gridDim.x);
+                for (int kb0 = 0; ok && kb0 < p.num_k_blocks; kb0 += U) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int kb = kb0 + u;
+                        if (kb >= p.num_k_blocks) break;
+                        if (!mbar_wait(&acc_empty[buf], bph ^ 1u, abort_flag)) { ok = false; break; }
+                        float* s = scale_s + (buf * C::GROUPS + g) * 128 + lane;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[32 * i] = x[u][i] * w[u];
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_full[buf]);
+                        if (kb + U < p.num_k_blocks) fetch(xs, ws, there, kb + U, x[u], w[u]);
+                        else if (more) fetch(xs_next, ws_next, there_next, u, x[u], w[u]);
+                        if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+                    }
                 }
             }
         }
@@ -196,36 +233,12 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         float* bias_s = reinterpret_cast<float*>(smem + C::BIAS_OFFSET) + ew * COLS;
         const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_first;
         const bool res = p.epilogue == B200_EPI_BIAS_RESIDUAL;
-        uint32_t buf = 0, bph = 0, rph = 0;
+        uint32_t buf = 0, bph = 0, st = 0, rph = 0;
         bool ok = true;
-        // The scales of this thread's row and of the warp's columns, fetched two k-blocks ahead, over the end of a tile too:
-        // their way from L2 is longer than a k-block (fetched one ahead, 16384 x 4096 x 4096 on 128-wide tiles took 556 us, so 373).
-        struct Ahead {
-            int tile, kb;
-            const float *xs, *ws;
-        } at = {group - num_groups, 0, nullptr, nullptr};
-        auto next_tile = [&]() {
-            at.tile += num_groups;
-            at.kb = 0;
-            const int r = at.tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-            const int b = (at.tile % p.num_n_tiles * BN + col_first) / fp8::kBlock;
-            at.xs = p.x_scale + (r < p.M ? r : 0);
-            at.ws = p.w_scale + static_cast<long long>(b < p.w_blocks ? b : p.w_blocks - 1) * p.num_k_blocks;
-        };
-        auto fetch_scales = [&](float& x, float& w) {
-            if (at.tile >= p.num_tiles) return;
-            x = __ldg(at.xs);
-            w = __ldg(at.ws);
-            at.xs += p.ld_xs;
-            ++at.ws;
-            if (++at.kb == p.num_k_blocks) next_tile();
-        };
-        float x_s[2] = {0.f, 0.f}, w_s[2] = {0.f, 0.f};
-        next_tile();
-        fetch_scales(x_s[0], w_s[0]);
-        fetch_scales(x_s[1], w_s[1]);
-        for (int tile = group; ok && tile < p.num_tiles; tile += num_groups) {
-            const int row0 = tile / p.num_n_tiles * (128 * CG) + static_cast<int>(rank) * 128 + quarter * 32;
+        const float* my_scale = scale_s + col_first / 128 * 128 + quarter * 32 + lane;
+        const uint32_t first_lane = lane == 0;
+        for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+            const int row0 = tile / p.num_n_tiles * 128 + quarter * 32;
             const int n_first = tile % p.num_n_tiles * BN + col_first;
             // what this warp stores of the tile: 64-column pieces of its 32 rows (the store clips what lies outside y)
             const int pieces = row0 < p.M && n_first < p.N ? min(COLS / 64, (p.N - n_first + 63) / 64) : 0;
@@ -240,37 +253,41 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             uint64_t acc[COLS / 2];
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
-            for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-                const float scale = x_s[0] * w_s[0];
-                const uint64_t s2 = pack_f32x2(scale, scale);
-                x_s[0] = x_s[1];
-                w_s[0] = w_s[1];
-                fetch_scales(x_s[1], w_s[1]);
-                if (!mbar_wait(&acc_full[buf], bph, abort_flag)) { ok = false; break; }
+            // 32 columns travel while the 32 before them are added, across k-blocks too: the chain of wait, load, release of one
+            // warp is what bounds a k-block.
+            uint32_t r[2][32];
+            float scale = 0.f;
+            auto open = [&]() -> bool {   // the next buffer: its first 32 columns and its scale
+                if (!mbar_wait(&acc_full[buf], bph, abort_flag)) return false;
                 __syncwarp();
                 tcgen05_fence_after();
-                // 32 columns travel while the 32 before them are added
-                uint32_t r[2][32];
                 tmem_ld_32x32b_x32(tacc + buf * BN, r[0]);
+                scale = my_scale[buf * (C::GROUPS * 128)];
+                return true;
+            };
+            ok = open();
+#pragma unroll 1
+            for (int kb = 0; ok && kb < p.num_k_blocks; ++kb) {
+                const uint64_t s2 = pack_f32x2(scale, scale);
 #pragma unroll
                 for (int c = 0; c < COLS / 32; ++c) {
                     tmem_ld_wait(r[c & 1]);
                     if (c + 1 < COLS / 32) {
                         tmem_ld_32x32b_x32(tacc + buf * BN + (c + 1) * 32, r[(c + 1) & 1]);
-                    } else {   // the buffer is in registers: hand it back
+                    } else {   // the buffer is in registers: hand it back, and the stage
                         tcgen05_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
-                            if (CG == 2 && !leader) mbar_arrive_leader(&acc_empty[buf]);
-                            else mbar_arrive(&acc_empty[buf]);
-                        }
+                        mbar_arrive_if(&acc_empty[buf], first_lane);
+                        mbar_arrive_if(&empty[st], first_lane & (ew == 0));
+                        if (++st == STAGES) st = 0;
+                        if (++buf == NBUF) { buf = 0; bph ^= 1u; }
+                        if (kb + 1 < p.num_k_blocks) ok = open();
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         acc[c * 16 + j] = fma_f32x2(pack_f32x2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), s2,
                                                     acc[c * 16 + j]);
                 }
-                if (++buf == NBUF) { buf = 0; bph ^= 1u; }
                 if (kb == 0 && res && pieces > 0 && lane == 0) {
                     // the residual of this tile into the strips, which the previous tile's stores have read by now
                     tma_store_wait_read<0>();
@@ -435,86 +452,26 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     // ---------------------------------------------------------------- teardown
     tcgen05_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync_all();   // neither CTA frees TMEM or leaves while the other may still signal or read it
     if (warp == 1) {
         tcgen05_fence_after();
-        if (CG == 2) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
-        else tmem_dealloc(tmem_base, C::TMEM_COLS);
+        tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
     if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) atomicOr(p.status, 1u);
 }
 
-// Launch with a cluster dimension (CG = 2) beside the programmatic-serialization attribute.
-template <int CG, typename... KArgs, typename... Args>
-cudaError_t launch_groups(void (*kernel)(KArgs...), unsigned ctas, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl_enabled()) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (CG == 2) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 2;
-        attr[n].val.clusterDim.y = 1;
-        attr[n++].val.clusterDim.z = 1;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = static_cast<unsigned>(n);
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
-// CTA groups that can be resident at once (a persistent grid must not exceed it), looked up once per device and instance.
-template <int CG, int BN, int EW, int OUT>
-int resident_groups(int sms) {
-    using C = Fp8Cfg<CG, BN, EW>;
-    static PerDeviceOnce once;
-    static int groups[kMaxDevices];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    const bool ready = once.ensure(dev, [&]() {
-        if (cudaFuncSetAttribute(linear_fp8_kernel<CG, BN, EW, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
-            cudaSuccess) {
-            cudaGetLastError();
-            return false;
-        }
-        int n = sms;
-        if (CG == 2) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
-            cfg.blockDim = dim3(C::THREADS);
-            cfg.dynamicSmemBytes = C::SMEM_BYTES;
-            cudaLaunchAttribute attr;
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = 2;
-            attr.val.clusterDim.y = 1;
-            attr.val.clusterDim.z = 1;
-            cfg.attrs = &attr;
-            cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, linear_fp8_kernel<CG, BN, EW, OUT>, &cfg) != cudaSuccess || n <= 0) {
-                cudaGetLastError();
-                n = sms / 2;
-            }
-            if (n > sms / 2) n = sms / 2;
-        }
-        groups[dev] = n;
-        return true;
-    });
-    return ready ? groups[dev] : 0;
-}
-
-template <int CG, int BN, int EW, int OUT>
+template <int BN, int EW, int OUT>
 int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) {
-    using C = Fp8Cfg<CG, BN, EW>;
-    const int groups = resident_groups<CG, BN, EW, OUT>(sms);
-    if (groups <= 0) return B200_ERR_LAUNCH;
+    using C = Fp8Cfg<BN, EW>;
+    static PerDeviceOnce once;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return B200_ERR_LAUNCH;
+    if (!once.ensure(dev, []() {
+            return cudaFuncSetAttribute(linear_fp8_kernel<BN, EW, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) ==
+                   cudaSuccess;
+        }))
+        return B200_ERR_LAUNCH;
     // Rows that do not exist are not fetched where all rows fit one box: what the stage holds there feeds no stored row.
-    const int x_rows = CG == 1 && d.M < 128 ? static_cast<int>((d.M + 7) / 8 * 8) : 128;
+    const int x_rows = d.M < 128 ? static_cast<int>((d.M + 7) / 8 * 8) : 128;
     CUtensorMap tx, tw, ty, tr;
     {   // two e4m3 values as one 16-bit element
         const uint64_t xd[2] = {static_cast<uint64_t>(d.K / 2), static_cast<uint64_t>(d.M)};
@@ -522,7 +479,7 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
         const uint32_t xb[2] = {64, static_cast<uint32_t>(x_rows)};
         const uint64_t wd[2] = {static_cast<uint64_t>(d.K / 2), static_cast<uint64_t>(d.N)};
         const uint64_t ws[1] = {static_cast<uint64_t>(d.ldw)};
-        const uint32_t wb[2] = {64, BN / CG};
+        const uint32_t wb[2] = {64, BN};
         const uint64_t cols = OUT == kOutF32 ? 2 * static_cast<uint64_t>(d.N) : (OUT == kOutF8 ? d.N / 2 : d.N);
         const uint64_t yd[2] = {cols, static_cast<uint64_t>(d.M)};
         const uint64_t ys[1] = {static_cast<uint64_t>(d.ldy) * (OUT == kOutF32 ? 4 : (OUT == kOutF8 ? 1 : 2))};
@@ -543,7 +500,7 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
     p.M = static_cast<int>(d.M);
     p.N = static_cast<int>(d.N);
     p.num_n_tiles = (p.N + BN - 1) / BN;
-    const long long tiles = (d.M + 128 * CG - 1) / (128 * CG) * p.num_n_tiles;
+    const long long tiles = (d.M + 127) / 128 * p.num_n_tiles;
     if (tiles > 0x7fffffffll) return B200_ERR_UNSUPPORTED;
     p.num_tiles = static_cast<int>(tiles);
     p.num_k_blocks = static_cast<int>((d.K + 127) / 128);
@@ -554,25 +511,24 @@ int launch_linear_fp8(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) 
     p.epilogue = d.epilogue;
     p.ld_xs = d.ld_x_scale;
     p.ld_ys = d.ld_y_scale;
-    p.idesc = make_idesc_f16(128 * CG, BN, 0, 0, 0);   // format code 0 of kind::f8f6f4 = e4m3
+    p.idesc = make_idesc_f16(128, BN, 0, 0, 0);   // format code 0 of kind::f8f6f4 = e4m3
     p.status = device_status_ptr();
-    const int used = p.num_tiles < groups ? p.num_tiles : groups;
-    launch_groups<CG>(linear_fp8_kernel<CG, BN, EW, OUT>, static_cast<unsigned>(used * CG), C::THREADS, C::SMEM_BYTES, stream, tx, tw,
-                      ty, tr, p);
+    const dim3 grid(static_cast<unsigned>(p.num_tiles < sms ? p.num_tiles : sms));
+    launch_kernel(linear_fp8_kernel<BN, EW, OUT>, grid, dim3(C::THREADS), C::SMEM_BYTES, stream, tx, tw, ty, tr, p);
     count_launch();
     return check_launch();
 }
 
-template <int CG, int BN>
+template <int BN>
 int launch_by_output(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) {
     // e4m3 output: a thread holds a whole scale block of its row, 128 columns
     constexpr int EW = BN == 64 ? 4 : 8, EW8 = BN == 256 ? 8 : 4;
     if (d.out_dtype == B200_E4M3) {
-        if constexpr (BN >= 128) return launch_linear_fp8<CG, BN, EW8, kOutF8>(d, stream, sms);
+        if constexpr (BN >= 128) return launch_linear_fp8<BN, EW8, kOutF8>(d, stream, sms);
         else return B200_ERR_PARAM;
     }
-    if (d.out_dtype == B200_F32) return launch_linear_fp8<CG, BN, EW, kOutF32>(d, stream, sms);
-    return launch_linear_fp8<CG, BN, EW, kOutHalf>(d, stream, sms);
+    if (d.out_dtype == B200_F32) return launch_linear_fp8<BN, EW, kOutF32>(d, stream, sms);
+    return launch_linear_fp8<BN, EW, kOutHalf>(d, stream, sms);
 }
 
 int validate_linear_fp8(const B200LinearFp8Desc* d) {
@@ -590,7 +546,7 @@ int validate_linear_fp8(const B200LinearFp8Desc* d) {
     if (d->epilogue == B200_EPI_BIAS_RESIDUAL &&
         (!d->residual || !is_half_dtype(d->res_dtype) || (d->ldr % 8) || d->ldr < d->N || !aligned16(d->residual)))
         return B200_ERR_PARAM;
-    if (d->block_n != 0 && d->block_n != 128 && d->block_n != 256 && d->block_n != -128 && (d->block_n != -64 || f8)) return B200_ERR_PARAM;
+    if (d->block_n != 0 && d->block_n != 128 && d->block_n != 256 && (d->block_n != 64 || f8)) return B200_ERR_PARAM;
     return B200_OK;
 }
 
@@ -607,11 +563,10 @@ extern "C" int b200_linear_fp8_fwd(const B200LinearFp8Desc* d, b200_stream_t str
     if (sms <= 0) return B200_ERR_NOT_SM100;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     int bn = d->block_n;
-    if (bn == 0) bn = d->M <= 128 ? (d->out_dtype == B200_E4M3 ? -128 : -64) : 256;
+    if (bn == 0) bn = d->M <= 128 ? (d->out_dtype == B200_E4M3 ? 128 : 64) : 256;
     switch (bn) {
-        case 256: return launch_by_output<2, 256>(*d, stream, sms);
-        case 128: return launch_by_output<2, 128>(*d, stream, sms);
-        case -128: return launch_by_output<1, 128>(*d, stream, sms);
-        default: return launch_by_output<1, 64>(*d, stream, sms);
+        case 256: return launch_by_output<256>(*d, stream, sms);
+        case 128: return launch_by_output<128>(*d, stream, sms);
+        default: return launch_by_output<64>(*d, stream, sms);
     }
 }

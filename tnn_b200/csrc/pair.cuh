@@ -70,15 +70,6 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t tmem_d, uint64_t desc_
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_f8_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                                uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 // One arrival on the barrier at this shared-memory offset in both CTAs of the pair once all UMMAs issued so far are done.
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
     const uint16_t mask = 3;
@@ -86,11 +77,6 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
         ::"r"(smem_u32(bar)), "h"(mask)
         : "memory");
-}
-// The commits of kernels whose UMMAs are umma_f8_*, on a pair or on one CTA.
-__device__ __forceinline__ void umma_f8_commit(uint64_t* bar, bool pair) {
-    if (pair) umma_commit_pair(bar);
-    else umma_commit(bar);
 }
 __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
     asm volatile(

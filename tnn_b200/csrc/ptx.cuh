@@ -35,6 +35,12 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// The same under a predicate, without a branch.
+__device__ __forceinline__ void mbar_arrive_if(uint64_t* bar, uint32_t on) {
+    asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.u32 P, %1, 0;\n\t@P mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n"
+                 ::"r"(smem_u32(bar)), "r"(on)
+                 : "memory");
+}
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -197,6 +203,9 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
+
+// The commit of kernels whose UMMAs are umma_f8_*.
+__device__ __forceinline__ void umma_f8_commit(uint64_t* bar) { umma_commit(bar); }
 
 // TMEM -> registers: lane (base lane + threadIdx%32), 32 consecutive 32-bit columns starting at taddr's column.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
