@@ -7,8 +7,10 @@
 // short as the run needs, in steps of 32 keys (QK^T with N = 32 c, PV with K = 32 c, c chunks of softmax), so that four sinks
 // cost a quarter of a tile.
 //
-// tcgen05 (S = Q K^T, O += P V), one softmax warpgroup, online softmax with lazy maximum; persistent CTAs, two per SM, so
-// that one's exp pass covers the other's hand-offs.
+// tcgen05 (S = Q K^T, O += P V), one softmax warpgroup, online softmax with lazy maximum; two CTAs per SM, so that one's exp
+// pass covers the other's hand-offs.  How long an item takes depends on its sequence's length and on its place in it, so items
+// are not dealt in advance: the grid has a CTA per item, and a running CTA takes over the next one that has not started
+// (cluster launch control), prefetching its queries and scores while it is still at work on its own.
 #include "linear_common.cuh"
 #include "ptx.cuh"
 #include "window.cuh"
@@ -24,7 +26,7 @@ constexpr float kLazyLog2 = 8.0f;            // the running maximum moves only w
 
 struct TileParams : WindowParams {
     uint32_t idesc_qk, idesc_pv;             // idesc_qk without its N field
-    int n_qb, n_items;
+    int n_qb;
 };
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -34,6 +36,7 @@ struct TileParams : WindowParams {
 //   warp 1     : UMMA issuer (one elected lane): S(j + 1) before PV(j), across items;
 //   warp 2     : zeroes the V rows of a tile that no query may see (beyond the run, or dropped by the mask): their weight is
 //                exactly 0, but 0 x NaN is not;
+//   warp 3     : takes over items and hands their numbers to the others through a ring of kIds;
 //   warps 4..7 : softmax, thread = query row.
 // TMEM: S 128 columns, O 64, P 64 (half precision, the A operand of PV).
 struct WCfg {
@@ -45,17 +48,45 @@ struct WCfg {
     static constexpr int OFF_V = OFF_K + NST * TILE_BYTES;
     static constexpr int OFF_MASK = OFF_V + NST * TILE_BYTES;      // NST x 128 floats
     static constexpr int OFF_BITS = OFF_MASK + NST * TK * 4;       // NST x 4 words
-    static constexpr int OFF_BAR = OFF_BITS + NST * 16;
-    static constexpr int SMEM = OFF_BAR + 256;
+    static constexpr int OFF_TAKEN = OFF_BITS + NST * 16;          // 16 bytes: the answer of a take-over
+    static constexpr int kIds = 2;                                 // items on their way to the other roles
+    static constexpr int OFF_ITEMS = OFF_TAKEN + 16;               // kIds x 32 bytes
+    static constexpr int OFF_BAR = OFF_ITEMS + kIds * 32;
+    static constexpr int SMEM = OFF_BAR + 384;
+    static constexpr int kReaders = 7;                             // producer, issuer, V rows, four softmax warps
     static constexpr int TMEM_COLS = 256, COL_O = 128, COL_P = 192;
 };
 static_assert(128 * WCfg::REGS_CONTROL + 128 * WCfg::REGS_SOFTMAX <= 65536 / 2, "setmaxnreg moves registers inside the CTA's own share");
 
-struct WItem {
+struct __align__(16) WItem {
     int b, head, q0, p0;      // p0: position of the item's first query
-    int a_end, b_lo, b_hi;
-    int n_a, n;               // tiles of the first run, of both
+    int a_end, b_lo, b_hi;    // the runs
+    int there;                // 0: no further item
+    __device__ __forceinline__ int tiles_a() const { return (a_end + TK - 1) / TK; }
+    __device__ __forceinline__ int tiles() const { return tiles_a() + (b_hi - b_lo + TK - 1) / TK; }
 };
+
+// Asks for the first CTA of the grid that has not started; the answer arrives in shared memory and completes 16 bytes of `bar`.
+__device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
+                 : "memory");
+}
+// Its block index, or -1 if every CTA has started.
+__device__ __forceinline__ int taken_over(const void* answer) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return ok ? static_cast<int>(x) : -1;
+}
 struct WTile {
     int k0, end, chunks;      // first key, end of its run, 32-key chunks
 };
@@ -72,29 +103,30 @@ __device__ __forceinline__ WItem load_item(const TileParams& p, int id) {
     it.a_end = r.a_end;
     it.b_lo = r.b_lo;
     it.b_hi = r.b_hi;
-    it.n_a = (r.a_end + TK - 1) / TK;
-    it.n = it.n_a + (r.b_hi - r.b_lo + TK - 1) / TK;
+    it.there = 1;
     return it;
 }
 __device__ __forceinline__ WTile load_tile(const WItem& it, int j) {
     WTile t;
-    t.k0 = j < it.n_a ? j * TK : it.b_lo + (j - it.n_a) * TK;
-    t.end = j < it.n_a ? it.a_end : it.b_hi;
+    const int n_a = it.tiles_a();
+    t.k0 = j < n_a ? j * TK : it.b_lo + (j - n_a) * TK;
+    t.end = j < n_a ? it.a_end : it.b_hi;
     t.chunks = (min(TK, t.end - t.k0) + 31) >> 5;
     return t;
 }
 
-// MASKED: with an additive key mask
+// MASKED: scores are scaled (and given their additive mask, if there is one) before the maximum: with a mask, or a scale that is
+// not positive; otherwise the scale is folded into the exponential.
 template <int DT, bool MASKED>
 __global__ void __launch_bounds__(WCfg::THREADS, 2)
 window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                        const __grid_constant__ CUtensorMap tm_v, const TileParams p) {
+                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const TileParams p) {
     using C = WCfg;
     constexpr int NST = C::NST;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* q_full = bars;                 // [2]
-    uint64_t* q_free = q_full + 2;           // [2] the item's last QK^T has read its queries
+    uint64_t* q_free = q_full + 2;           // [2] the item's output, staged in the place of its queries, has been read
     uint64_t* k_full = q_free + 2;           // [NST]
     uint64_t* v_full = k_full + NST;
     uint64_t* v_ready = v_full + NST;        // the rows that nobody may see are zero
@@ -105,8 +137,12 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     uint64_t* s_free = s_full + 1;           // the scores are in registers (128 arrivals)
     uint64_t* p_full = s_free + 1;           // 128 arrivals
     uint64_t* o_full = p_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+    uint64_t* taken = o_full + 1;
+    uint64_t* id_full = taken + 1;           // [kIds]
+    uint64_t* id_free = id_full + C::kIds;   // [kIds], a reader's arrival each
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(id_free + C::kIds);
     volatile uint32_t* abort_flag = tmem_slot + 1;
+    WItem* items = reinterpret_cast<WItem*>(smem + C::OFF_ITEMS);   // [kIds]
     float* mask_s = reinterpret_cast<float*>(smem + C::OFF_MASK);
     uint32_t* bits_s = reinterpret_cast<uint32_t*>(smem + C::OFF_BITS);
 
@@ -118,7 +154,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 1);
-            mbar_init(&q_free[i], 1);
+            mbar_init(&q_free[i], 4);
         }
         for (int i = 0; i < NST; ++i) {
             mbar_init(&k_full[i], 1);
@@ -132,6 +168,11 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         mbar_init(s_free, 128);
         mbar_init(p_full, 128);
         mbar_init(o_full, 1);
+        mbar_init(taken, 1);
+        for (int i = 0; i < C::kIds; ++i) {
+            mbar_init(&id_full[i], 1);
+            mbar_init(&id_free[i], C::kReaders);
+        }
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tm_q);
@@ -149,8 +190,26 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     pdl_launch_dependents();
     pdl_wait();   // q, k, v, kv_len and q_start come from earlier kernels; the output may still be read by one
 
-    const int id0 = blockIdx.x, id_step = gridDim.x;
     constexpr bool masked = MASKED;
+    // The CTA's next item; `n` counts the caller's reads.  A warp reads as one (lane 0 arrives), the issuer is a single thread.
+    auto next_item = [&](uint32_t& n, WItem& it) -> bool {
+        const uint32_t slot = n % C::kIds;
+        if (!mbar_wait(&id_full[slot], (n / C::kIds) & 1u, abort_flag)) return false;
+        it = items[slot];
+        mbar_arrive(&id_free[slot]);
+        ++n;
+        return it.there != 0;
+    };
+    auto next_item_warp = [&](uint32_t& n, WItem& it) -> bool {
+        const uint32_t slot = n % C::kIds;
+        const bool ok = mbar_wait(&id_full[slot], (n / C::kIds) & 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        it = items[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&id_free[slot]);
+        ++n;
+        return it.there != 0;
+    };
     // Items without a visible key have no tiles: only the softmax warpgroup, which writes their zeros, stops at them.  `k`
     // counts the others (query set and phase), `t` tiles (ring stage and phase).
     if (warp < 4) {
@@ -158,10 +217,11 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (warp == 0) {
             // ------------------------------------------------------------ producer
             bool ok = true;
-            uint32_t k = 0, t = 0;
-            for (int id = id0; ok && id < p.n_items; id += id_step) {
-                const WItem it = load_item(p, id);
-                if (it.n == 0) continue;
+            uint32_t k = 0, t = 0, n = 0;
+            WItem it;
+            while (ok && next_item_warp(n, it)) {
+                const int n_tiles = it.tiles();
+                if (n_tiles == 0) continue;
                 const int kv_col = it.head / p.group * HD;
                 const uint32_t set = k & 1u;
                 if (!mbar_wait(&q_free[set], ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
@@ -170,7 +230,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     tma_load_3d(smem + C::OFF_Q + set * TILE_BYTES, &tm_q, &q_full[set], it.head * HD, it.q0, it.b);
                 }
                 ++k;
-                for (int j = 0; j < it.n; ++j, ++t) {
+                for (int j = 0; j < n_tiles; ++j, ++t) {
                     const WTile tl = load_tile(it, j);
                     const int st = static_cast<int>(t % NST);
                     const uint32_t ph = ((t / NST) & 1u) ^ 1u;
@@ -190,13 +250,13 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             const int key = tl.k0 + c * 32 + lane;
                             float m = 0.f;
                             bool seen = false;
-                            if (key < tl.end) {
+                            if (key < tl.end && p.mask_add != nullptr) {
                                 m = p.mask_add[static_cast<long long>(it.b) * p.Sk + key];
                                 seen = m > p.mask_below;
                             }
                             mask_s[st * TK + c * 32 + lane] = seen ? m * kLog2e : 0.f;
                             const uint32_t word = __ballot_sync(0xffffffffu, seen);
-                            if (lane == 0) bits_s[st * 4 + c] = word;
+                            if (lane == 0) bits_s[st * 4 + c] = p.mask_add != nullptr ? word : 0xFFFFFFFFu;
                         }
                         mbar_arrive(&m_full[st]);
                     }
@@ -227,7 +287,6 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     for (int e = 0; e < HD / 16; ++e) umma_f16_ss(tmem_base, a + 2u * e, b + 2u * e, idesc, e != 0 ? 1u : 0u);
                     umma_commit(s_full);
                     umma_commit(&k_empty[st]);
-                    if (j == it.n - 1) umma_commit(&q_free[k & 1u]);
                     ++n_s;
                     return true;
                 };
@@ -246,25 +305,36 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     ++n_pv;
                     return true;
                 };
-                auto next = [&](int id, WItem& it) -> int {   // the first item at or after `id` that has tiles
-                    for (; id < p.n_items; id += id_step) {
-                        it = load_item(p, id);
-                        if (it.n != 0) return id;
+                uint32_t n = 0;
+                // The next item that has tiles: 1 found, 0 there is none, and, unless `wait`, -1: not known yet.  It must not be
+                // waited for with a tile's PV outstanding: the softmax warps read on in the ring only when their item is done.
+                auto next = [&](WItem& it, bool wait) -> int {
+                    for (;;) {
+                        const uint32_t slot = n % C::kIds;
+                        if (!wait && !mbar_try_wait(&id_full[slot], (n / C::kIds) & 1u)) return -1;
+                        if (!next_item(n, it)) return 0;
+                        if (it.tiles() != 0) return 1;
                     }
-                    return id;
                 };
                 WItem it, it_n;
                 uint32_t k = 0;
-                int id = next(id0, it);
-                bool ok = id >= p.n_items || issue_s(it, 0, k);
-                while (ok && id < p.n_items) {
-                    const int id_n = next(id + id_step, it_n);
-                    for (int j = 0; ok && j < it.n; ++j) {
-                        if (j + 1 < it.n) ok = issue_s(it, j + 1, k);
-                        else if (id_n < p.n_items) ok = issue_s(it_n, 0, k + 1);
+                int there = next(it, true);
+                bool ok = there != 1 || issue_s(it, 0, k);
+                while (ok && there == 1) {
+                    const int n_tiles = it.tiles();
+                    for (int j = 0; ok && j < n_tiles; ++j) {
+                        if (j + 1 < n_tiles) {   // the following scores before this tile's PV
+                            ok = issue_s(it, j + 1, k);
+                        } else {
+                            there = next(it_n, false);
+                            if (there == 1) ok = issue_s(it_n, 0, k + 1);
+                        }
                         ok = ok && issue_pv(it, j);
+                        if (ok && there == -1) {
+                            there = next(it_n, true);
+                            if (there == 1) ok = issue_s(it_n, 0, k + 1);
+                        }
                     }
-                    id = id_n;
                     it = it_n;
                     ++k;
                 }
@@ -273,10 +343,11 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         } else if (warp == 2) {
             // ------------------------------------------------------------ V rows that nobody may see
             bool ok = true;
-            uint32_t t = 0;
-            for (int id = id0; ok && id < p.n_items; id += id_step) {
-                const WItem it = load_item(p, id);
-                for (int j = 0; j < it.n; ++j, ++t) {
+            uint32_t t = 0, n = 0;
+            WItem it;
+            while (ok && next_item_warp(n, it)) {
+                const int n_tiles = it.tiles();
+                for (int j = 0; j < n_tiles; ++j, ++t) {
                     const WTile tl = load_tile(it, j);
                     const int st = static_cast<int>(t % NST);
                     const uint32_t ph = (t / NST) & 1u;
@@ -307,6 +378,28 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 }
             }
             __syncwarp();
+        } else {
+            // ------------------------------------------------------------ items: this CTA's own, then those it takes over
+            if (elect_one()) {
+                int id = blockIdx.x;
+                for (uint32_t n = 0;; ++n) {
+                    const uint32_t slot = n % C::kIds;
+                    // the next one is asked for while this one is looked up
+                    if (id >= 0) {
+                        mbar_expect_tx(taken, 16);
+                        take_over(smem + C::OFF_TAKEN, taken);
+                    }
+                    if (!mbar_wait(&id_free[slot], ((n / C::kIds) & 1u) ^ 1u, abort_flag)) break;
+                    WItem it = {};
+                    if (id >= 0) it = load_item(p, id);
+                    items[slot] = it;
+                    mbar_arrive(&id_full[slot]);
+                    if (id < 0) break;   // every CTA has started: not asked again
+                    if (!mbar_wait(taken, n & 1u, abort_flag)) break;
+                    id = taken_over(smem + C::OFF_TAKEN);
+                }
+            }
+            __syncwarp();
         }
     } else {
         setmaxnreg_inc<C::REGS_SOFTMAX>();
@@ -314,20 +407,28 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const int r_in_tile = tid - 128;
         const uint32_t t_s = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_o = t_s + C::COL_O, t_p = t_s + C::COL_P;
-        uint32_t t = 0;
-        bool ok = true;
-        for (int id = id0; ok && id < p.n_items; id += id_step) {
-            const WItem it = load_item(p, id);
-            const int rows = min(TQ, p.Sq - it.q0);
-            const int pos = it.p0 + r_in_tile;
-            const int kv_lo = pos - p.left, kv_hi = pos + p.right;   // the row's window
+        uint32_t t = 0, n = 0, k = 0;
+        bool ok = true, staged = false;   // staged: item k - 1's output is on its way out of query set (k - 1) & 1
+        WItem it;
+        while (ok && next_item_warp(n, it)) {
+            const int n_tiles = it.tiles();
+            if (n_tiles == 0) {   // no key: zeros
+                const int q = it.q0 + r_in_tile;
+                uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_batch + q * p.ldo + it.head * HD;
+                if (q < p.Sq)
+                    for (int g = 0; g < HD / 8; ++g) *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(0, 0, 0, 0);
+                continue;
+            }
+            // what every row of the item sees: keys [all_lo, all_hi] (and the first tokens); what this row does
+            const int all_lo = it.p0 + min(TQ, p.Sq - it.q0) - 1 - p.left, all_hi = it.p0 + p.right;
+            const int row_lo = it.p0 + r_in_tile - p.left, row_hi = it.p0 + r_in_tile + p.right;
             float m_run = -INFINITY, l_run = 0.f;
-            for (int j = 0; j < it.n; ++j, ++t) {
+            for (int j = 0; j < n_tiles; ++j, ++t) {
                 const WTile tl = load_tile(it, j);
                 const int st = static_cast<int>(t % NST);
                 // every key of the tile visible to every row
-                const bool plain = !masked && p.scale_log2 > 0.f && tl.end - tl.k0 >= TK &&
-                                   (tl.k0 + TK <= p.sinks || (tl.k0 >= it.p0 + rows - 1 - p.left && tl.k0 + TK - 1 <= it.p0 + p.right));
+                const bool plain = !masked && tl.end - tl.k0 >= TK &&
+                                   (tl.k0 + TK <= p.sinks || (tl.k0 >= all_lo && tl.k0 + TK - 1 <= all_hi));
                 if (masked && !mbar_wait(&m_full[st], (t / NST) & 1u, abort_flag)) { ok = false; break; }
                 if (!mbar_wait(s_full, t & 1u, abort_flag)) { ok = false; break; }
                 __syncwarp();
@@ -342,42 +443,38 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 tcgen05_fence_before();
                 mbar_arrive(s_free);
                 float tmx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (plain) {
 #pragma unroll
-                    for (int g = 0; g < TK / 8; ++g) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            tmx[c] = fmax3(tmx[c], __uint_as_float(s[g * 8 + c * 2]), __uint_as_float(s[g * 8 + c * 2 + 1]));
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < tl.chunks) {
+                for (int c = 0; c < 4; ++c) {
+                    if (c < tl.chunks) {
+                        // Hidden keys become -inf; a chunk that hides nothing from any row of the warp is left alone.  (Kept
+                        // small: an edge's code runs once in several tiles, and as a second copy of the whole pass, scaling
+                        // included, it took 2400 to 4700 clocks, most of them instruction fetches; the pass itself 300.)
+                        if (!plain) {
                             const int k0 = tl.k0 + c * 32;
-                            uint32_t bits = (low_bits(kv_hi + 1 - k0) & ~low_bits(kv_lo - k0)) | low_bits(p.sinks - k0);
+                            uint32_t bits = (low_bits(row_hi + 1 - k0) & ~low_bits(row_lo - k0)) | low_bits(p.sinks - k0);
                             bits &= low_bits(tl.end - k0);
-                            if (masked) {
+                            if (masked && p.mask_add != nullptr) {
                                 bits &= bits_s[st * 4 + c];
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const float x = fmaf(__uint_as_float(s[c * 32 + e]), p.scale_log2, mask_s[st * TK + c * 32 + e]);
-                                    s[c * 32 + e] = __float_as_uint((bits >> e) & 1u ? x : -INFINITY);
-                                }
-                            } else {
+                                for (int e = 0; e < 32; ++e)
+                                    s[c * 32 + e] = __float_as_uint(fmaf(__uint_as_float(s[c * 32 + e]), p.scale_log2, mask_s[st * TK + c * 32 + e]));
+                            } else if (masked) {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const float x = __uint_as_float(s[c * 32 + e]) * p.scale_log2;
-                                    s[c * 32 + e] = __float_as_uint((bits >> e) & 1u ? x : -INFINITY);
-                                }
+                                for (int e = 0; e < 32; ++e) s[c * 32 + e] = __float_as_uint(__uint_as_float(s[c * 32 + e]) * p.scale_log2);
                             }
+                            if (__any_sync(0xffffffffu, bits != 0xFFFFFFFFu)) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2)
-                                tmx[(e >> 1) & 3] = fmax3(tmx[(e >> 1) & 3], __uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1]));
+                                for (int e = 0; e < 32; ++e)
+                                    if ((bits & (1u << e)) == 0) s[c * 32 + e] = 0xFF800000u;
+                            }
                         }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2)
+                            tmx[(e >> 1) & 3] = fmax3(tmx[(e >> 1) & 3], __uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1]));
                     }
                 }
                 float tmax = fmaxf(fmaxf(tmx[0], tmx[1]), fmaxf(tmx[2], tmx[3]));
-                if (plain) tmax *= p.scale_log2;
+                if (!masked) tmax *= p.scale_log2;   // (positive: other scales take the masked form)
                 const bool move = tmax > m_run + kLazyLog2;
                 const float m_new = move ? tmax : m_run;
                 const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
@@ -397,7 +494,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                         tmem_st_32x32b_x16(t_o + c * 16, ro);
                     }
                 }
-                const float mul = plain ? p.scale_log2 : 1.f;
+                const float mul = masked ? 1.f : p.scale_log2;
                 const uint64_t mul2 = pack_f32x2(mul, mul), neg2 = pack_f32x2(-m_use, -m_use);
                 uint64_t ps2[2] = {0ull, 0ull};
 #pragma unroll
@@ -425,37 +522,53 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 tmem_st_wait();
                 tcgen05_fence_before();
                 mbar_arrive(p_full);
+                if (j == 0 && staged) {   // the previous item's output has had this tile's time to leave
+                    if (lane == 0) {
+                        tma_store_wait_read<0>();
+                        mbar_arrive(&q_free[(k - 1) & 1u]);
+                    }
+                    __syncwarp();
+                    staged = false;
+                }
             }
             if (!ok) break;
-            if (it.n > 0 && !mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
+            if (!mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
             __syncwarp();
             tcgen05_fence_after();
+            // The output takes the place of the item's queries (its last QK^T is long done) and leaves by TMA, 32 rows of a warp at
+            // a time, clipped at row Sq.  (Stored from registers, 16 bytes of 32 rows per instruction, it held the warps up for
+            // 1600 to 3700 clocks an item.)
             // l_run is 0 where no key was visible (a sum of weights is at least the maximum's 2^-8), NaN where a score was
             const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-            const int q = it.q0 + r_in_tile;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_batch + q * p.ldo + it.head * HD;
+            uint8_t* strip = smem + C::OFF_Q + (k & 1u) * TILE_BYTES + (warp & 3) * 32 * 128;
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t r[32];
-                if (it.n > 0) {
-                    tmem_ld_32x32b_x32(t_o + c * 32, r);
-                    tmem_ld_wait(r);
-                }
-                if (q < p.Sq) {
-                    const bool none = it.n == 0 || l_run == 0.f;
+                tmem_ld_32x32b_x32(t_o + c * 32, r);
+                tmem_ld_wait(r);
+                const bool none = l_run == 0.f;
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        uint4 qv;
-                        qv.x = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 0]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
-                        qv.y = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
-                        qv.z = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
-                        qv.w = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c * 32 + g * 8) = qv;
-                    }
+                for (int g = 0; g < 4; ++g) {
+                    uint4 qv;
+                    qv.x = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 0]) * inv, __uint_as_float(r[g * 8 + 1]) * inv);
+                    qv.y = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 2]) * inv, __uint_as_float(r[g * 8 + 3]) * inv);
+                    qv.z = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 4]) * inv, __uint_as_float(r[g * 8 + 5]) * inv);
+                    qv.w = none ? 0u : pack2t<DT>(__uint_as_float(r[g * 8 + 6]) * inv, __uint_as_float(r[g * 8 + 7]) * inv);
+                    *reinterpret_cast<uint4*>(strip + lane * 128 + (((c * 4 + g) ^ (lane & 7)) << 4)) = qv;
                 }
             }
+            fence_async_proxy_shared();
+            __syncwarp();
+            if (lane == 0 && it.q0 + (warp & 3) * 32 < p.Sq) {
+                tma_store_3d(&tm_o, strip, it.head * HD, it.q0 + (warp & 3) * 32, it.b);
+                tma_store_commit();
+            }
+            staged = true;
+            ++k;
             tcgen05_fence_before();
         }
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
     }
 
     tcgen05_fence_before();
@@ -541,7 +654,6 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     const long long items = n_qb * d->heads * d->B;
     if (items > 0x7fff0000ll) return B200_ERR_UNSUPPORTED;
     p.n_qb = static_cast<int>(n_qb);
-    p.n_items = static_cast<int>(items);
     const int fmt = d->dtype == B200_BF16 ? 1 : 0;
     p.idesc_qk = make_idesc_f16(TQ, 0, fmt, 0, 0);
     p.idesc_pv = make_idesc_f16(TQ, HD, fmt, 0, 1);   // V is MN-major
@@ -552,17 +664,18 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     const uint64_t qs[2] = {static_cast<uint64_t>(d->ldq) * 2, static_cast<uint64_t>(p.q_batch) * 2};
     const uint64_t ks[2] = {static_cast<uint64_t>(d->ldk) * 2, static_cast<uint64_t>(p.k_batch) * 2};
     const uint64_t vs[2] = {static_cast<uint64_t>(d->ldv) * 2, static_cast<uint64_t>(p.v_batch) * 2};
-    CUtensorMap tq, tk, tv;
+    const uint64_t os[2] = {static_cast<uint64_t>(d->ldo) * 2, static_cast<uint64_t>(p.o_batch) * 2};
+    const uint32_t strip[3] = {HD, 32, 1};
+    CUtensorMap tq, tk, tv, to;
     if (!get_tensor_map(&tq, d->q, 3, qd, qs, box) || !get_tensor_map(&tk, d->k, 3, kd, ks, box) ||
-        !get_tensor_map(&tv, d->v, 3, kd, vs, box))
+        !get_tensor_map(&tv, d->v, 3, kd, vs, box) || !get_tensor_map(&to, d->out, 3, qd, os, strip))
         return B200_ERR_DRIVER;
     if (!set_window_attributes(dev)) return B200_ERR_LAUNCH;
-    const long long slots = 2ll * sms;
-    const dim3 grid(static_cast<unsigned>(items < slots ? items : slots));
-    const bool masked = d->mask_add != nullptr;
+    const dim3 grid(static_cast<unsigned>(items));
+    const bool masked = d->mask_add != nullptr || !(d->scale > 0.f);
     auto kernel = d->dtype == B200_F16 ? (masked ? window_attention_kernel<B200_F16, true> : window_attention_kernel<B200_F16, false>)
                                        : (masked ? window_attention_kernel<B200_BF16, true> : window_attention_kernel<B200_BF16, false>);
-    launch_kernel(kernel, grid, dim3(WCfg::THREADS), WCfg::SMEM, stream, tq, tk, tv, p);
+    launch_kernel(kernel, grid, dim3(WCfg::THREADS), WCfg::SMEM, stream, tq, tk, tv, to, p);
     count_launch();
     return check_launch();
 }
