@@ -257,6 +257,33 @@ def test_linear_fp8_rows_do_not_depend_on_the_batch_or_the_tile(cuda_device):
 
 
 @pytest.mark.parametrize("out", [F16, F32, F8])
+@pytest.mark.parametrize("epi", ["bias", "residual"])
+@pytest.mark.parametrize("M,N,block_n", [(30000, 328, 256), (30000, 264, 256), (20000, 200, 128), (20000, 72, 64)])
+def test_linear_fp8_many_tiles_per_cta_with_a_ragged_last_column(cuda_device, M, N, block_n, epi, out):
+    """Tiles of unequal width follow one another on a CTA: an output strip is written again only when its store has read it."""
+    if out == F8 and (block_n == 64 or N % 16):
+        block_n, N = 128, N // 16 * 16
+    x8, xs, w8, ws = _operands(cuda_device, M, N, 144, 11)
+    bias = _randn(cuda_device, 1, N)
+    res = _randn(cuda_device, 2, M, N).to(F16) if epi == "residual" else None
+    code = ops.EPI_BIAS if res is None else ops.EPI_BIAS_RESIDUAL
+    got = ops.linear_fp8(x8, xs, w8, ws, bias, residual=res, epilogue=code, out_dtype=out, block_n=block_n)
+    for r in (slice(0, 200), slice(M // 2, M // 2 + 300), slice(M - 100, M)):      # one tile per CTA: no strip is used twice
+        part = ops.linear_fp8(x8[r], xs[:, r].contiguous(), w8, ws, bias, residual=None if res is None else res[r], epilogue=code,
+                              out_dtype=out, block_n=block_n)
+        if out == F8:
+            assert torch.equal(part[0].view(torch.uint8), got[0][r].view(torch.uint8)) and torch.equal(part[1], got[1][:, r])
+        else:
+            assert torch.equal(part, got[r])
+    want, size = _product(x8, xs, w8, ws)
+    want = want + bias.double() + (0 if res is None else res.double())
+    y = values(*got) if out == F8 else got.double()
+    step = 0 if out != F8 else got[1].t().double().repeat_interleave(128, 1)[:, :N] * 2.0 ** -10
+    bound = HALF_STEP[out] * want.abs() * 1.01 + step + 1e-4 * (size + bias.double().abs() + (0 if res is None else res.double().abs()))
+    assert bool(((y - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("out", [F16, F32, F8])
 @pytest.mark.parametrize("M,N,block_n", [(1, 80, 0), (41, 272, 128), (300, 272, 256), (130, 144, 128)])
 def test_linear_fp8_strides_and_what_lies_around_the_output(cuda_device, M, N, block_n, out):
     K = 272

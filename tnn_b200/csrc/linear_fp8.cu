@@ -254,7 +254,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         float* bias_s = reinterpret_cast<float*>(smem + C::BIAS_OFFSET) + ew * COLS;
         const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + col_first;
         const bool res = p.epilogue == B200_EPI_BIAS_RESIDUAL;
-        uint32_t buf = 0, bph = 0, st = 0, rph = 0;
+        uint32_t buf = 0, bph = 0, st = 0, rph = 0, stored = 0;   // stored: strips sent off, the two in turn
         bool ok = true;
         const float* my_scale = scale_s + col_first / 128 * 128 + quarter * 32 + lane;
         const uint32_t first_lane = lane == 0;
@@ -372,9 +372,10 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
 #pragma unroll
                 for (int h = 0; h < COLS / 64; ++h) {
                     if (h >= pieces) break;
-                    uint8_t* srow = strips + h * C::STRIP_BYTES + lane * 128;
-                    if (!res) {   // the strip's store of the previous tile has read it
-                        if (lane == 0) tma_store_wait_read<COLS / 64 - 1>();
+                    uint8_t* strip = strips + (res ? h : (stored++ & 1u)) * C::STRIP_BYTES;
+                    uint8_t* srow = strip + lane * 128;
+                    if (!res) {   // the store before the last one has read its strip
+                        if (lane == 0) tma_store_wait_read<1>();
                         __syncwarp();
                     }
 #pragma unroll
@@ -394,7 +395,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                     fence_async_proxy_shared();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_2d(&tm_y, strips + h * C::STRIP_BYTES, n_first + h * 64, row0);
+                        tma_store_2d(&tm_y, strip, n_first + h * 64, row0);
                         tma_store_commit();
                     }
                 }
@@ -418,7 +419,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
                         if (n_first + c * 32 >= p.N) break;
-                        uint8_t* srow = strips + (c & 1) * C::STRIP_BYTES + lane * 128;
+                        uint8_t* strip = strips + (stored++ & 1u) * C::STRIP_BYTES;
+                        uint8_t* srow = strip + lane * 128;
                         float v[32];
                         if (res) {
 #pragma unroll
@@ -426,7 +428,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         } else {
                             finish(c, v);
                         }
-                        if (lane == 0) tma_store_wait_read<1>();   // the strip's last store has read it
+                        if (lane == 0) tma_store_wait_read<1>();   // the store before the last one has read its strip
                         __syncwarp();
 #pragma unroll
                         for (int g = 0; g < 8; ++g)
@@ -434,7 +436,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         fence_async_proxy_shared();
                         __syncwarp();
                         if (lane == 0) {
-                            tma_store_2d(&tm_y, strips + (c & 1) * C::STRIP_BYTES, 2 * (n_first + c * 32), row0);
+                            tma_store_2d(&tm_y, strip, 2 * (n_first + c * 32), row0);
                             tma_store_commit();
                         }
                     }
