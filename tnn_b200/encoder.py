@@ -23,14 +23,25 @@ class Encoder:
         self._ws = None
         self._ws_key = None
         self.fold = False
+        self.fp8 = False          # matrix weights in block-scaled e4m3
+        self.window = None        # (left, right): sliding-window attention
+        self.sinks = 0
 
     @classmethod
-    def from_workload(cls, wl, dtype=torch.float16, device="cuda", fold_layernorm=False):
+    def from_workload(cls, wl, dtype=torch.float16, device="cuda", fold_layernorm=False, fp8=False, window=None, sinks=0):
         """`fold_layernorm`: prepare the weights for the five-launch form of a layer (both LayerNorms folded into
         the neighbouring GEMMs); only full encoder layers can be folded.  Off by default: at BERT's K = 768 the
-        seven-launch layer with its own LayerNorm kernel is the faster one, and it is what the TNN plug-in runs."""
+        seven-launch layer with its own LayerNorm kernel is the faster one, and it is what the TNN plug-in runs.
+
+        For long documents: `fp8` keeps the matrix weights in e4m3 with a scale per 128 x 128 block and runs the four GEMMs
+        of a layer on 8-bit operands (activations between launches stay in `dtype`, the feed-forward's inner one in 8 bits);
+        `window=(left, right)` lets every token see that many neighbours and the first `sinks` tokens only.  A sequence whose
+        keys are all masked then yields an attention output of zeros."""
         enc = cls(wl.cfg, dtype, torch.device(device))
         enc.fold = bool(fold_layernorm) and wl.cfg.with_ffn
+        enc.fp8, enc.window, enc.sinks = bool(fp8), window, int(sinks)
+        if enc.fold and (enc.fp8 or window is not None):
+            raise ValueError("fold_layernorm is a form of the half-precision, full-attention layer")
         H, F = wl.cfg.hidden, wl.cfg.ffn
 
         def dev(a):
@@ -39,6 +50,9 @@ class Encoder:
         prev = None
         for lw in wl.weights:
             L = {}
+            if enc.fp8:
+                enc.layers.append(cls._fp8_layer(lw, wl.cfg, dev))
+                continue
             w_qkv = torch.empty((3 * H, H), dtype=dtype, device=enc.device)
             L["b_qkv"] = dev(np.concatenate([lw.bq, lw.bk, lw.bv]))
             if enc.fold and prev is not None:
@@ -68,32 +82,78 @@ class Encoder:
         torch.cuda.synchronize(enc.device)
         return enc
 
+    @staticmethod
+    def _fp8_layer(lw, cfg, dev):
+        L = {"b_qkv": dev(np.concatenate([lw.bq, lw.bk, lw.bv])), "b_o": dev(lw.bo), "ln1_g": dev(lw.ln1_g), "ln1_b": dev(lw.ln1_b)}
+        L["w_qkv"] = ops.pack_weight_fp8(dev(np.concatenate([lw.wq, lw.wk, lw.wv], axis=1)))   # (codes, scales)
+        L["w_o"] = ops.pack_weight_fp8(dev(lw.wo))
+        if cfg.with_ffn:
+            L["w_ffn1"], L["w_ffn2"] = ops.pack_weight_fp8(dev(lw.w1)), ops.pack_weight_fp8(dev(lw.w2))
+            L["b_ffn1"], L["b_ffn2"] = dev(lw.b1), dev(lw.b2)
+            L["ln2_g"], L["ln2_b"] = dev(lw.ln2_g), dev(lw.ln2_b)
+        return L
+
+    def _attention(self, qkv, m2, kv_len):
+        cfg = self.cfg
+        scale = 1.0 / float(np.sqrt(cfg.head_dim))
+        if self.window is None:
+            return ops.attention(qkv, cfg.heads, m2, kv_len, scale=scale)
+        H = cfg.hidden
+        return ops.window_attention(qkv[..., :H], qkv[..., H:2 * H], qkv[..., 2 * H:], cfg.heads, window=self.window,
+                                    sinks=self.sinks, mask_add=m2, kv_len=kv_len, scale=scale)
+
+    def _fp8_stack(self, h, m2, kv_len, out=None):
+        """The layers on 8-bit operands: h `[B,S,H]` half precision -> the same; nine launches a layer and a quantizer in
+        front of the first.  Every LayerNorm also writes the 8-bit operand of the GEMMs behind it."""
+        cfg = self.cfg
+        codes, scales = ops.quantize_fp8(h)
+        last = self.layers[-1] if self.layers else None
+        for L in self.layers:
+            end = L is last
+            qkv = ops.linear_fp8(codes, scales, *L["w_qkv"], L["b_qkv"], out_dtype=self.dtype)
+            ctx = ops.quantize_fp8(self._attention(qkv, m2, kv_len))
+            t = ops.linear_fp8(*ctx, *L["w_o"], L["b_o"], residual=h, epilogue=ops.EPI_BIAS_RESIDUAL, out_dtype=self.dtype)
+            if end and not cfg.with_ffn:
+                return ops.add_layernorm(t, L["ln1_g"], L["ln1_b"], cfg.ln_eps, out=out)
+            h, codes, scales = ops.add_layernorm_fp8(t, L["ln1_g"], L["ln1_b"], cfg.ln_eps)
+            if not cfg.with_ffn:
+                continue
+            f1 = ops.linear_fp8(codes, scales, *L["w_ffn1"], L["b_ffn1"], epilogue=ops.EPI_BIAS_GELU, out_dtype=torch.float8_e4m3fn)
+            t = ops.linear_fp8(*f1, *L["w_ffn2"], L["b_ffn2"], residual=h, epilogue=ops.EPI_BIAS_RESIDUAL, out_dtype=self.dtype)
+            if end:
+                return ops.add_layernorm(t, L["ln2_g"], L["ln2_b"], cfg.ln_eps, out=out)
+            h, codes, scales = ops.add_layernorm_fp8(t, L["ln2_g"], L["ln2_b"], cfg.ln_eps)
+        return h
+
     # ------------------------------------------------------------------ layer-by-layer path (any config)
     def forward_ops(self, x_f32, mask_add=None, out_f32=True):
         """x_f32 `[B,S,H]` fp32 device tensor -> `[B,S,H]`; one launch per fused layer."""
         if self.fold:
             return self._forward_ops_folded(x_f32, mask_add, out_f32)
-        cfg = self.cfg
         B, S, H = x_f32.shape
         h = ops.convert(x_f32.contiguous(), self.dtype)
-        kv_len = None
-        m2 = None
+        m2 = kv_len = None
         if mask_add is not None:
             m2 = mask_add.reshape(B, S).contiguous()
             kv_len = ops.mask_to_kv_len(m2)
-        scale = 1.0 / float(np.sqrt(cfg.head_dim))
+        h = self._fp8_stack(h, m2, kv_len) if self.fp8 else self._half_stack(h, m2, kv_len)
+        return ops.convert(h, torch.float32) if out_f32 else h
+
+    def _half_stack(self, h, m2, kv_len, out=None):
+        cfg = self.cfg
         for L in self.layers:
+            end = out if L is self.layers[-1] else None
             qkv = ops.linear(h, L["w_qkv"], L["b_qkv"])
-            ctx = ops.attention(qkv, cfg.heads, m2, kv_len, scale=scale)
+            ctx = self._attention(qkv, m2, kv_len)
             t = ops.linear(ctx, L["w_o"], L["b_o"], residual=h, epilogue=ops.EPI_BIAS_RESIDUAL)
-            a = ops.add_layernorm(t, L["ln1_g"], L["ln1_b"], cfg.ln_eps)
+            a = ops.add_layernorm(t, L["ln1_g"], L["ln1_b"], cfg.ln_eps, out=None if cfg.with_ffn else end)
             if cfg.with_ffn:
                 f1 = ops.linear(a, L["w_ffn1"], L["b_ffn1"], epilogue=ops.EPI_BIAS_GELU)
                 t2 = ops.linear(f1, L["w_ffn2"], L["b_ffn2"], residual=a, epilogue=ops.EPI_BIAS_RESIDUAL)
-                h = ops.add_layernorm(t2, L["ln2_g"], L["ln2_b"], cfg.ln_eps)
+                h = ops.add_layernorm(t2, L["ln2_g"], L["ln2_b"], cfg.ln_eps, out=end)
             else:
                 h = a
-        return ops.convert(h, torch.float32) if out_f32 else h
+        return h
 
     def _forward_ops_folded(self, x_f32, mask_add, out_f32):
         """The five-launch layer, one C-ABI call per launch (what b200_encoder_fwd does with fold_layernorm = 1)."""
@@ -159,9 +219,13 @@ class Encoder:
         return self._ws.data_ptr() + off
 
     def forward_hidden(self, hidden, mask2d=None, kv_len=None):
-        """In-place stack over `hidden` `[B,S,H]` (fp16/bf16 device tensor) through b200_encoder_fwd."""
+        """In-place stack over `hidden` `[B,S,H]` (fp16/bf16 device tensor) through b200_encoder_fwd (8-bit weights and
+        windows: through the operators)."""
         if not self.cfg.with_ffn:
             raise ValueError("b200_encoder_fwd runs full encoder layers; use forward_ops for attention-only blocks")
+        if self.fp8 or self.window is not None:   # launch by launch; the last LayerNorm writes the result in place
+            (self._fp8_stack if self.fp8 else self._half_stack)(hidden, mask2d, kv_len, out=hidden)
+            return hidden
         B, S, H = hidden.shape
         d = capi.EncoderDesc(hidden.data_ptr(), capi.ptr(mask2d), capi.ptr(kv_len), self._layer_array(),
                              self.workspace(B * S), B, S, H, self.cfg.ffn, self.cfg.heads, len(self.layers),
