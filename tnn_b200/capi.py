@@ -197,10 +197,11 @@ def ptr(t):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream_ptr():
+def stream_ptr(device=None):
+    """The current stream of device number `device` (None: of the current device)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch.cuda.current_device() if device is None else device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def device_status():

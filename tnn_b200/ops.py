@@ -253,10 +253,10 @@ def _call(name, desc, index):
     if fn is None:
         fn = _entry[name] = getattr(capi.lib(), name)
     if index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(desc), capi.stream_ptr())
+        rc = fn(ctypes.byref(desc), capi.stream_ptr(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(ctypes.byref(desc), capi.stream_ptr())
+            rc = fn(ctypes.byref(desc), capi.stream_ptr(index))
     if rc != capi.OK:
         capi.check(rc, name)
 
@@ -272,10 +272,9 @@ def _device_index(x, *ts):
     return index
 
 
-def _new(shape, dtype, device):
-    """Uninitialised contiguous tensor of two or three dimensions (empty_strided costs 1.5 us of host time, empty 2.4)."""
-    strides = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
-    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+def _new(rows, cols, dtype, device):
+    """Uninitialised contiguous matrix (empty_strided costs 1.5 us of host time, empty 2.4)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def _new_like(x, dtype):
@@ -340,7 +339,7 @@ def quantize_fp8(x, out=None, out_scale=None):
         _codes(out, x.shape, "out")
         q, ldq = _out_rows(out, K, rows, "out")
     if out_scale is None:
-        out_scale = _new((blocks, rows), torch.float32, x.device)
+        out_scale = _new(blocks, rows, torch.float32, x.device)
         lds = rows
     else:
         lds = _scale_rows(out_scale, blocks, rows, "out_scale")
@@ -358,11 +357,11 @@ def pack_weight_fp8(w_kn, out=None, out_scale=None):
         raise ValueError("w_kn: fp32 [K, N], contiguous columns")
     K, N = w_kn.shape
     if out is None:
-        out = _new((N, K), _F8, w_kn.device)
+        out = _new(N, K, _F8, w_kn.device)
     _codes(out, (N, K), "out")
     w, ldw = _out_rows(out, K, N, "out")
     if out_scale is None:
-        out_scale = _new((_blocks(N), _blocks(K)), torch.float32, w_kn.device)
+        out_scale = _new(_blocks(N), _blocks(K), torch.float32, w_kn.device)
     if out_scale.dtype != torch.float32 or out_scale.shape != (_blocks(N), _blocks(K)) or not out_scale.is_contiguous():
         raise ValueError("out_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
     with torch.cuda.device(index):
@@ -396,7 +395,7 @@ def add_layernorm_fp8(x, gamma, beta, eps, residual=None, out=None, out8=None, o
         _codes(out8, x.shape, "out8")
         q, ldq = _out_rows(out8, H, rows, "out8")
     if out_scale is None:
-        out_scale = _new((blocks, rows), torch.float32, x.device)
+        out_scale = _new(blocks, rows, torch.float32, x.device)
         lds = rows
     else:
         lds = _scale_rows(out_scale, blocks, rows, "out_scale")
@@ -428,24 +427,25 @@ def linear_fp8(x8, x_scale, w8, w_scale, bias=None, residual=None, epilogue=EPI_
         ldw = w8.stride(0) if N > 1 else K
     else:
         raise ValueError("w8: [N, K] with contiguous rows")
-    if w_scale.dtype != torch.float32 or w_scale.shape != (_blocks(N), _blocks(K)) or not w_scale.is_contiguous():
-        raise ValueError("w_scale: contiguous fp32 [%d, %d]" % (_blocks(N), _blocks(K)))
+    kb, nb = -(-K // FP8_BLOCK), -(-N // FP8_BLOCK)
+    if w_scale.dtype != torch.float32 or w_scale.shape != (nb, kb) or not w_scale.is_contiguous():
+        raise ValueError("w_scale: contiguous fp32 [%d, %d]" % (nb, kb))
     _vector(bias, N, "bias")
     x2, M, ldx = _rows(x8, K)
-    ldxs = _scale_rows(x_scale, _blocks(K), M, "x_scale")
+    ldxs = _scale_rows(x_scale, kb, M, "x_scale")
     if out is not None:
         out_dtype = out.dtype
         y, ldy = _out_rows(out, N, M, "out")
     else:
-        out = (_new((M, N), out_dtype, x8.device) if x8.dim() == 2
+        out = (_new(M, N, out_dtype, x8.device) if x8.dim() == 2
                else torch.empty(x8.shape[:-1] + (N,), dtype=out_dtype, device=x8.device))
         y, ldy = out.data_ptr(), N
     f8 = out_dtype == _F8
     ys, ldys = None, 0
     if f8:
         if out_scale is None:
-            out_scale = _new((_blocks(N), M), torch.float32, x8.device)
-        ldys = _scale_rows(out_scale, _blocks(N), M, "out_scale")
+            out_scale = _new(nb, M, torch.float32, x8.device)
+        ldys = _scale_rows(out_scale, nb, M, "out_scale")
         ys = out_scale.data_ptr()
     r, ldr, r_code = None, 0, capi.F16
     if residual is not None:
@@ -461,16 +461,17 @@ def linear_fp8(x8, x_scale, w8, w_scale, bias=None, residual=None, epilogue=EPI_
 
 
 # ---------------------------------------------------------------------------- sliding-window attention
-def _heads_view(t, heads, what):
-    """(row stride, batch stride) of a `[B, S, heads * 64]` tensor whose heads lie side by side."""
-    if t.dim() != 3 or t.shape[2] != heads * 64:
-        raise ValueError("%s: [B, S, %d]" % (what, heads * 64))
+def _heads_view(t, S, W, what):
+    """(row stride, batch stride) of a `[B, S, W]` tensor whose heads lie side by side (strides of single rows or sequences mean
+    nothing)."""
     if t.is_contiguous():
-        return heads * 64, t.shape[1] * heads * 64
-    if t.stride(2) != 1:
+        return W, S * W
+    batch, ld, one = t.stride()
+    if one != 1:
         raise ValueError("%s: contiguous heads" % what)
-    ld = t.stride(1) if t.shape[1] > 1 else heads * 64
-    return ld, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * ld)
+    if S <= 1:
+        ld = W
+    return ld, (batch if t.shape[0] > 1 else S * ld)
 
 
 def _per_sequence(t, B, what):
@@ -493,29 +494,33 @@ def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, ma
     index = _device_index(q, k, v, mask_add, kv_len, q_start, out)
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads or sinks < 0:
         raise ValueError("kv_heads divides heads, sinks >= 0")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise ValueError("q, k, v: one dtype")
-    ldq, q_batch = _heads_view(q, heads, "q")
-    ldk, k_batch = _heads_view(k, kv_heads, "k")
-    ldv, v_batch = _heads_view(v, kv_heads, "v")
-    B, Sq, _ = q.shape
-    Bk, Sk, _ = k.shape
-    if Bk != B or v.shape != k.shape:
-        raise ValueError("k, v: [%d, Sk, %d]" % (B, kv_heads * 64))
+    W, Wk = heads * 64, kv_heads * 64
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q [B, Sq, %d], k, v [B, Sk, %d]" % (W, Wk))
+    B, Sq, Wq = q.shape
+    Bk, Sk, W_k = k.shape
+    if Wq != W or W_k != Wk or Bk != B or v.shape != k.shape:
+        raise ValueError("q [B, Sq, %d], k, v [B, Sk, %d]" % (W, Wk))
+    ldq, q_batch = _heads_view(q, Sq, W, "q")
+    ldk, k_batch = _heads_view(k, Sk, Wk, "k")
+    ldv, v_batch = _heads_view(v, Sk, Wk, "v")
     _per_sequence(kv_len, B, "kv_len")
     _per_sequence(q_start, B, "q_start")
     if out is None:
-        out = _new((B, Sq, heads * 64), q.dtype, q.device)
-        ldo, o_batch = heads * 64, Sq * heads * 64
+        out = torch.empty_strided((B, Sq, W), (Sq * W, W, 1), dtype=dtype, device=q.device)
+        ldo, o_batch = W, Sq * W
     else:
-        if out.dtype != q.dtype or out.shape != q.shape:
+        if out.dtype != dtype or out.shape != q.shape:
             raise ValueError("out: the dtype and shape of q")
-        ldo, o_batch = _heads_view(out, heads, "out")
+        ldo, o_batch = _heads_view(out, Sq, W, "out")
     if mask_add is not None and not (mask_add.dtype == torch.float32 and mask_add.numel() == B * Sk and mask_add.is_contiguous()):
         raise ValueError("mask_add: contiguous fp32 [%d, %d]" % (B, Sk))
     d = capi.WindowAttentionDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), capi.ptr(mask_add), capi.ptr(kv_len), capi.ptr(q_start),
                                  out.data_ptr(), B, Sq, Sk, ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch, window[0],
-                                 window[1], sinks, heads, kv_heads, 64, capi.dtype_code(q.dtype), 0.125 if scale is None else scale,
+                                 window[1], sinks, heads, kv_heads, 64, capi.dtype_code(dtype), 0.125 if scale is None else scale,
                                  exclude_below)
     if B and Sq:
         _call("b200_window_attention_fwd", d, index)
