@@ -14,6 +14,7 @@
 //   warps 4 ..  : EW epilogue warps: scale and add, then bias / activation / residual and the store
 #include "fp8.cuh"
 #include "linear_common.cuh"
+#include "linear_fp8.cuh"
 
 namespace b200 {
 namespace lin {
@@ -21,27 +22,6 @@ namespace lin {
 namespace {
 
 enum { kOutHalf = 0, kOutF32 = 1, kOutF8 = 2 };
-
-// GELU, x Phi(x) = max(x, 0) - u Q(u) with u = |x| and the normal tail Q(u) = exp(-u^2 / 2) P(u).  P, half the Mills ratio scaled
-// by sqrt(2 / pi), is smooth; a polynomial of degree 7 fitted to it on [0, 6] with the weight u exp(-u^2 / 2) leaves the result
-// 3.0e-6 off at most over all x (evaluated in fp32; the tail beyond 6 is under 6e-9).  The tanh form that half-precision results
-// get away with (3e-5, tanh.approx) moved enough e4m3 codes to show: error of a feed-forward pair 6.9e-4 with it, 2.8e-4 exact.
-// One MUFU instruction per value, everything else on packed pairs.  x + |x| keeps a NaN.
-__device__ __forceinline__ void gelu_tail_x2(float& a, float& b) {
-    const float ua = fabsf(a), ub = fabsf(b);
-    const uint64_t u = pack_f32x2(fminf(ua, 6.0f), fminf(ub, 6.0f));
-    uint64_t q = pack_f32x2(-9.496552e-5f, -9.496552e-5f);
-    const float c[7] = {1.505126e-3f, -1.03997699e-2f, 4.23175171e-2f, -1.17116407e-1f, 2.42861018e-1f, -3.9737156e-1f, 4.99881923e-1f};
-#pragma unroll
-    for (int i = 0; i < 7; ++i) q = fma_f32x2(q, u, pack_f32x2(c[i], c[i]));
-    float ta, tb;
-    unpack_f32x2(mul_f32x2(mul_f32x2(u, u), pack_f32x2(-0.72134752f, -0.72134752f)), ta, tb);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ta) : "f"(ta));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(tb) : "f"(tb));
-    const uint64_t tail = mul_f32x2(mul_f32x2(q, pack_f32x2(ta, tb)), u);
-    const uint64_t sum = add_f32x2(pack_f32x2(a, b), pack_f32x2(ua, ub));
-    unpack_f32x2(fma_f32x2(tail, pack_f32x2(-1.f, -1.f), mul_f32x2(sum, pack_f32x2(0.5f, 0.5f))), a, b);
-}
 
 struct LinearFp8Params {
     const float* x_scale;
@@ -569,7 +549,8 @@ int validate_linear_fp8(const B200LinearFp8Desc* d) {
     if (d->epilogue == B200_EPI_BIAS_RESIDUAL &&
         (!d->residual || !is_half_dtype(d->res_dtype) || (d->ldr % 8) || d->ldr < d->N || !aligned16(d->residual)))
         return B200_ERR_PARAM;
-    if (d->block_n != 0 && d->block_n != 128 && d->block_n != 256 && (d->block_n != 64 || f8)) return B200_ERR_PARAM;
+    if (d->block_n == -1 ? d->M > kFewRows : (d->block_n != 0 && d->block_n != 128 && d->block_n != 256 && (d->block_n != 64 || f8)))
+        return B200_ERR_PARAM;
     return B200_OK;
 }
 
@@ -607,6 +588,7 @@ extern "C" int b200_linear_fp8_fwd(const B200LinearFp8Desc* d, b200_stream_t str
     const int sms = device_sm_count();
     if (sms <= 0) return B200_ERR_NOT_SM100;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (d->block_n < 0 || (d->block_n == 0 && few_rows_pay(*d, sms))) return launch_linear_fp8_rows(*d, stream, sms);
     switch (d->block_n ? d->block_n : choose_columns(*d, sms)) {
         case 256: return launch_by_output<256>(*d, stream, sms);
         case 128: return launch_by_output<128>(*d, stream, sms);
