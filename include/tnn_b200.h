@@ -373,9 +373,11 @@ B200_API int b200_linear_fp8_fwd(const B200LinearFp8Desc* desc, b200_stream_t st
  *   kv_len      : int32 [B], keys of each sequence (clamped to Sk; <= 0: none), or NULL (= Sk).
  *   q_start     : int32 [B], position of each sequence's first query, or NULL (= 0): Sq new tokens at the end of a cache
  *                 of kv_len keys have q_start = kv_len - Sq.
- *   mask_add    : fp32 [B, Sk] additive key mask or NULL.  A key whose value is <= mask_exclude_below (or NaN) is dropped.
- *   A query that sees no key yields a row of zeros.  K and V rows that no query of the sequence may see (at or beyond kv_len,
- *   or dropped by mask_add) may hold anything, infinities and NaN included.
+ *   mask_add    : fp32 [B, Sk] additive key mask or NULL.  A key whose value is <= mask_exclude_below, <= -2^127 or
+ *                 NaN is dropped.
+ *   A query that sees no key yields a row of zeros.  K and V rows that no query of the sequence may see (outside every query's
+ *   window, at or beyond kv_len, or dropped by mask_add) may hold anything, infinities and NaN included; a row that some
+ *   query sees has to be finite for the others' results.
  *   q [B, Sq, ldq], k, v [B, Sk, ld*], out [B, Sq, ldo] : dtype (F16 / BF16), head h at columns h * 64; *_batch = elements
  *   from one sequence to the next.  Requirements: head_dim == 64, kv_heads divides heads, all strides % 8 == 0, 16-byte
  *   aligned pointers, Sq, Sk <= 2^24.

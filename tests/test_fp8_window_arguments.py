@@ -80,7 +80,7 @@ def _window(**kw):
 @pytest.mark.parametrize("kw", [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(B=-1), dict(Sq=-1), dict(Sk=0), dict(heads=0),
                                 dict(kv_heads=0), dict(kv_heads=3), dict(sinks=-1), dict(dtype=capi.F32), dict(dtype=capi.E4M3), dict(ldq=248),
                                 dict(ldq=260), dict(ldk=120), dict(ldv=100), dict(ldo=248), dict(q_batch=1284), dict(k_batch=0), dict(v_batch=-8),
-                                dict(o_batch=1024), dict(q=264), dict(k=264), dict(v=264), dict(out=264)])
+                                dict(o_batch=1024), dict(q=264), dict(k=264), dict(v=264), dict(out=264), dict(mask_add=256, mask_exclude_below=float("nan"))])
 def test_window_attention_refuses(kw):
     assert _window(**kw) == capi.ERR_PARAM
 

@@ -167,6 +167,38 @@ def test_places_that_nobody_may_see_hold_nan_and_infinities(cuda_device, Sq, Sk,
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("Sq", [1, 7, 70, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_cache_places_outside_every_window_hold_nan(cuda_device, Sq, dtype):
+    """Places given up behind the window and not yet written in front of it, with no kv_len to say so."""
+    starts = [611, 333, 0]
+    q, k, v, _, q_start, out = run(cuda_device, 3, Sq, 1000, 4, 2, (100, 0), 3, dtype, starts=starts)
+    k2, v2 = k.clone(), v.clone()
+    for b, p in enumerate(starts):
+        k2[b, 3:max(3, p - 100)], v2[b, 3:max(3, p - 100)] = math.nan, math.nan
+        k2[b, max(3, p + Sq):], v2[b, max(3, p + Sq):] = math.inf, math.nan
+    assert torch.equal(ops.window_attention(q, k2, v2, 4, 2, window=(100, 0), sinks=3, q_start=q_start), out)
+
+
+@pytest.mark.parametrize("Sq", [1, 150])
+def test_masks_of_the_lowest_value_with_no_threshold(cuda_device, Sq):
+    q, k, v = (_randn(cuda_device, i, 3, n, 128).half() for i, n in enumerate((Sq, 300, 300)))
+    lowest = torch.finfo(torch.float32).min
+    mask = torch.zeros(3, 300, device=cuda_device)
+    mask[0], mask[1, 100:] = lowest, lowest
+    mask[2], mask[2, 7], mask[2, 9] = -math.inf, -2.0 ** 126, -2.0 ** 126     # the only keys left: equal masks, of any size
+    out = ops.window_attention(q, k, v, 2, mask_add=mask, exclude_below=-math.inf)
+    assert bool((out[0] == 0).all())
+    drop = torch.zeros(3, 300, device=cuda_device)
+    drop[1, 100:] = -10000.0
+    drop[0], drop[2] = -10000.0, -10000.0
+    want, bound, _ = reference(q, k, v, 2, 2, (-1, -1), 0, drop)
+    check(out[1], want[1], bound[1])
+    # scores vanish beside 2^126, so the two weigh the same
+    mean = v[2, [7, 9]].double().mean(0)
+    assert bool(((out[2].double() - mean).abs() <= HALF_STEP[F16] * mean.abs() + 2.0 ** -24).all())
+
+
 @pytest.mark.parametrize("Sq,Sk", [(150, 150), (1, 600)])
 def test_packed_views_strided_cache_and_what_lies_around_the_output(cuda_device, Sq, Sk):
     heads, kv_heads, B = 4, 2, 3

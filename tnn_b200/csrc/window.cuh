@@ -30,6 +30,7 @@ struct WindowParams {
     int B;
     unsigned int* status;
 };
+constexpr float kLeastMask = -1.7014118e38f;  // -2^127: a mask at or below it is dropped whatever the threshold (x log2(e) it must stay finite)
 constexpr int kUnlimited = 1 << 28;          // beyond every position (Sq, Sk <= 2^24, q_start clamped to +-2^26)
 
 // The keys that queries at positions [p_first, p_last] of a sequence can see, as runs [0, a_end) and [b_lo, b_hi).

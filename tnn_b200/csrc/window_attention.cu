@@ -610,6 +610,7 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     if (d->B > 1 && (d->q_batch <= 0 || d->k_batch <= 0 || d->v_batch <= 0 || d->o_batch < (d->Sq - 1) * d->ldo + wq))
         return B200_ERR_PARAM;
     if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out)) return B200_ERR_PARAM;
+    if (d->mask_add && d->mask_exclude_below != d->mask_exclude_below) return B200_ERR_PARAM;
     if (d->B > 65535 || d->heads > 65535 || d->Sq > (1 << 24) || d->Sk > (1 << 24)) return B200_ERR_UNSUPPORTED;
     if (d->B == 0 || d->Sq == 0) return B200_OK;
     int dev = 0;
@@ -645,7 +646,7 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     p.right = side(d->right);
     p.sinks = d->sinks > d->Sk ? p.Sk : static_cast<int>(d->sinks);
     p.scale_log2 = d->scale * kLog2e;
-    p.mask_below = d->mask_exclude_below;
+    p.mask_below = d->mask_exclude_below > kLeastMask ? d->mask_exclude_below : kLeastMask;
     p.status = device_status_ptr();
 
     if (token_kernel_takes(p)) return launch_window_token(p, d->dtype, sms, stream);

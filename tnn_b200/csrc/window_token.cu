@@ -402,7 +402,7 @@ int launch_window_token(const WindowParams& p, int dtype, int sms, cudaStream_t 
     // 4 key / value heads, window 8192: 2 CTAs each 44.6 us, 4 (1.7 waves) 48.5, 8 56.4.)
     const int blocks = (p.Sq * p.group + kBlockRows - 1) / kBlockRows;
     const long long units = static_cast<long long>(p.B) * (p.heads / p.group) * blocks;
-    const long long reach = static_cast<long long>(p.left) + p.Sq + p.sinks;
+    const long long reach = static_cast<long long>(p.left) + p.right + p.Sq + p.sinks;
     const long long keys = p.Sk < reach ? p.Sk : reach;
     int ctas = 1;
     while (ctas < 8 && units * ctas * 2 <= 2ll * sms && keys >= 2ll * ctas * kWarps * kTile) ctas *= 2;

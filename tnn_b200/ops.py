@@ -488,7 +488,7 @@ def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, ma
     kv_len `[B]` int32: keys of each sequence (None: all Sk).  q_start `[B]` int32: position of each sequence's first query
     (None: 0); Sq new tokens at the end of a cache have q_start = kv_len - Sq.  mask_add fp32 `[B, Sk]`: additive key mask, a
     key at or below `exclude_below` is dropped.  A query that sees no key yields zeros; keys and values that no query may see
-    (beyond kv_len, or dropped) may hold anything."""
+    (outside every window, beyond kv_len, or dropped) may hold anything."""
     if kv_heads is None:
         kv_heads = heads
     index = _device_index(q, k, v, mask_add, kv_len, q_start, out)
