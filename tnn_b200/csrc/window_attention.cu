@@ -134,8 +134,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     uint64_t* v_empty = k_empty + NST;
     uint64_t* m_full = v_empty + NST;        // mask values and bits written (32 arrivals)
     uint64_t* s_full = m_full + NST;
-    uint64_t* s_free = s_full + 1;           // the scores are in registers (128 arrivals)
-    uint64_t* p_full = s_free + 1;           // 128 arrivals
+    uint64_t* s_free = s_full + 1;           // the scores are in registers (4 arrivals)
+    uint64_t* p_full = s_free + 1;           // 4 arrivals
     uint64_t* o_full = p_full + 1;
     uint64_t* taken = o_full + 1;
     uint64_t* id_full = taken + 1;           // [kIds]
@@ -165,8 +165,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             mbar_init(&m_full[i], 32);
         }
         mbar_init(s_full, 1);
-        mbar_init(s_free, 128);
-        mbar_init(p_full, 128);
+        mbar_init(s_free, 4);
+        mbar_init(p_full, 4);
         mbar_init(o_full, 1);
         mbar_init(taken, 1);
         for (int i = 0; i < C::kIds; ++i) {
@@ -421,58 +421,69 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             }
             // what every row of the item sees: keys [all_lo, all_hi] (and the first tokens); what this row does
             const int all_lo = it.p0 + min(TQ, p.Sq - it.q0) - 1 - p.left, all_hi = it.p0 + p.right;
+            // tiles [0, plain_a) and [plain_lo, plain_hi): every key visible to every row
+            const int n_a = it.tiles_a(), plain_a = masked ? 0 : it.a_end / TK;
+            const int plain_lo = n_a + (max(all_lo - it.b_lo, 0) + TK - 1) / TK;
+            const int plain_hi = masked ? 0 : n_a + max(min(it.b_hi, all_hi + 1) - it.b_lo, 0) / TK;
+            int k0 = n_a > 0 ? 0 : it.b_lo, end = n_a > 0 ? it.a_end : it.b_hi;
             const int row_lo = it.p0 + r_in_tile - p.left, row_hi = it.p0 + r_in_tile + p.right;
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n_tiles; ++j, ++t) {
-                const WTile tl = load_tile(it, j);
+                const WTile tl = {k0, end, (min(TK, end - k0) + 31) >> 5};
                 const int st = static_cast<int>(t % NST);
-                // every key of the tile visible to every row
-                const bool plain = !masked && tl.end - tl.k0 >= TK &&
-                                   (tl.k0 + TK <= p.sinks || (tl.k0 >= all_lo && tl.k0 + TK - 1 <= all_hi));
+                const bool plain = j < plain_a || (j >= plain_lo && j < plain_hi);
+                k0 += TK;
+                if (j + 1 == n_a) {
+                    k0 = it.b_lo;
+                    end = it.b_hi;
+                }
                 if (masked && !mbar_wait(&m_full[st], (t / NST) & 1u, abort_flag)) { ok = false; break; }
                 if (!mbar_wait(s_full, t & 1u, abort_flag)) { ok = false; break; }
                 __syncwarp();
                 tcgen05_fence_after();
-                uint32_t s[TK];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < tl.chunks) tmem_ld_32x32b_x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < tl.chunks) tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
-                tcgen05_fence_before();
-                mbar_arrive(s_free);
-                float tmx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c < tl.chunks) {
-                        // Hidden keys become -inf; a chunk that hides nothing from any row of the warp is left alone.  (Kept
-                        // small: an edge's code runs once in several tiles, and as a second copy of the whole pass, scaling
-                        // included, it took 2400 to 4700 clocks, most of them instruction fetches; the pass itself 300.)
-                        if (!plain) {
-                            const int k0 = tl.k0 + c * 32;
-                            uint32_t bits = (low_bits(row_hi + 1 - k0) & ~low_bits(row_lo - k0)) | low_bits(p.sinks - k0);
-                            bits &= low_bits(tl.end - k0);
-                            if (masked && p.mask_add != nullptr) {
+                // Hidden keys become -inf in TMEM, and so does what lies behind a short tile's last chunk; from there on all kinds
+                // of tiles share one path.  What bounds this kernel first is fetching instructions: with the edges' code in the
+                // passes below, unrolled four times over, and unrolled waits it was 69 KB long and took 150 us for 16384 causal
+                // queries of 16 heads, window 1024; 49 KB take 139.6.
+                if (!plain) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[32];
+                        const int first = tl.k0 + c * 32;
+                        uint32_t bits = (low_bits(row_hi + 1 - first) & ~low_bits(row_lo - first)) | low_bits(p.sinks - first);
+                        bits &= low_bits(tl.end - first);
+                        tmem_ld_32x32b_x32(t_s + c * 32, s);
+                        tmem_ld_wait(s);
+                        if (masked) {
+                            if (p.mask_add != nullptr) {
                                 bits &= bits_s[st * 4 + c];
 #pragma unroll
                                 for (int e = 0; e < 32; ++e)
-                                    s[c * 32 + e] = __float_as_uint(fmaf(__uint_as_float(s[c * 32 + e]), p.scale_log2, mask_s[st * TK + c * 32 + e]));
-                            } else if (masked) {
+                                    s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), p.scale_log2, mask_s[st * TK + c * 32 + e]));
+                            } else {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) s[c * 32 + e] = __float_as_uint(__uint_as_float(s[c * 32 + e]) * p.scale_log2);
-                            }
-                            if (__any_sync(0xffffffffu, bits != 0xFFFFFFFFu)) {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if ((bits & (1u << e)) == 0) s[c * 32 + e] = 0xFF800000u;
+                                for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * p.scale_log2);
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            tmx[(e >> 1) & 3] = fmax3(tmx[(e >> 1) & 3], __uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1]));
+                        for (int e = 0; e < 32; ++e)
+                            if ((bits & (1u << e)) == 0) s[e] = 0xFF800000u;
+                        tmem_st_32x32b_x32(t_s + c * 32, s);
                     }
+                    tmem_st_wait();
                 }
+                uint32_t s[TK];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+                tcgen05_fence_before();
+                __syncwarp();
+                mbar_arrive_if(s_free, lane == 0);
+                float tmx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < TK; e += 2)
+                    tmx[(e >> 1) & 3] = fmax3(tmx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                 float tmax = fmaxf(fmaxf(tmx[0], tmx[1]), fmaxf(tmx[2], tmx[3]));
                 if (!masked) tmax *= p.scale_log2;   // (positive: other scales take the masked form)
                 const bool move = tmax > m_run + kLazyLog2;
@@ -521,7 +532,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 m_run = m_new;
                 tmem_st_wait();
                 tcgen05_fence_before();
-                mbar_arrive(p_full);
+                __syncwarp();
+                mbar_arrive_if(p_full, lane == 0);
                 if (j == 0 && staged) {   // the previous item's output has had this tile's time to leave
                     if (lane == 0) {
                         tma_store_wait_read<0>();
