@@ -194,7 +194,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     // The CTA's next item; `n` counts the caller's reads.  A warp reads as one (lane 0 arrives), the issuer is a single thread.
     auto next_item = [&](uint32_t& n, WItem& it) -> bool {
         const uint32_t slot = n % C::kIds;
-        if (!mbar_wait(&id_full[slot], (n / C::kIds) & 1u, abort_flag)) return false;
+        if (!mbar_wait_small(&id_full[slot], (n / C::kIds) & 1u, abort_flag)) return false;
         it = items[slot];
         mbar_arrive(&id_free[slot]);
         ++n;
@@ -202,7 +202,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     };
     auto next_item_warp = [&](uint32_t& n, WItem& it) -> bool {
         const uint32_t slot = n % C::kIds;
-        const bool ok = mbar_wait(&id_full[slot], (n / C::kIds) & 1u, abort_flag);
+        const bool ok = mbar_wait_small(&id_full[slot], (n / C::kIds) & 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) return false;
         it = items[slot];
         __syncwarp();
@@ -224,7 +224,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 if (n_tiles == 0) continue;
                 const int kv_col = it.head / p.group * HD;
                 const uint32_t set = k & 1u;
-                if (!mbar_wait(&q_free[set], ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                if (!mbar_wait_small(&q_free[set], ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                 if (lane == 0) {
                     mbar_expect_tx(&q_full[set], TILE_BYTES);
                     tma_load_3d(smem + C::OFF_Q + set * TILE_BYTES, &tm_q, &q_full[set], it.head * HD, it.q0, it.b);
@@ -234,12 +234,12 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     const WTile tl = load_tile(it, j);
                     const int st = static_cast<int>(t % NST);
                     const uint32_t ph = ((t / NST) & 1u) ^ 1u;
-                    if (!mbar_wait(&k_empty[st], ph, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait_small(&k_empty[st], ph, abort_flag)) { ok = false; break; }
                     if (lane == 0) {
                         mbar_expect_tx(&k_full[st], TILE_BYTES);
                         tma_load_3d(smem + C::OFF_K + st * TILE_BYTES, &tm_k, &k_full[st], kv_col, tl.k0, it.b);
                     }
-                    if (!mbar_wait(&v_empty[st], ph, abort_flag)) { ok = false; break; }   // also: the stage's mask is done with
+                    if (!mbar_wait_small(&v_empty[st], ph, abort_flag)) { ok = false; break; }   // also: the stage's mask is done with
                     if (lane == 0) {
                         mbar_expect_tx(&v_full[st], TILE_BYTES);
                         tma_load_3d(smem + C::OFF_V + st * TILE_BYTES, &tm_v, &v_full[st], kv_col, tl.k0, it.b);
@@ -276,9 +276,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 // S of tile j of the CTA's k-th item, once the softmax has taken the scores in front of it
                 auto issue_s = [&](const WItem& it, int j, uint32_t k) -> bool {
                     const int st = static_cast<int>(n_s % NST);
-                    if (j == 0 && !mbar_wait(&q_full[k & 1u], (k >> 1) & 1u, abort_flag)) return false;
-                    if (!mbar_wait(&k_full[st], (n_s / NST) & 1u, abort_flag)) return false;
-                    if (!mbar_wait(s_free, (n_s & 1u) ^ 1u, abort_flag)) return false;
+                    if (j == 0 && !mbar_wait_small(&q_full[k & 1u], (k >> 1) & 1u, abort_flag)) return false;
+                    if (!mbar_wait_small(&k_full[st], (n_s / NST) & 1u, abort_flag)) return false;
+                    if (!mbar_wait_small(s_free, (n_s & 1u) ^ 1u, abort_flag)) return false;
                     tcgen05_fence_after();
                     const uint32_t idesc = p.idesc_qk | (static_cast<uint32_t>(load_tile(it, j).chunks * 4) << 17);
                     const uint64_t a = dq0 + static_cast<uint64_t>((k & 1u) * (TILE_BYTES >> 4));
@@ -292,8 +292,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 };
                 auto issue_pv = [&](const WItem& it, int j) -> bool {
                     const int st = static_cast<int>(n_pv % NST);
-                    if (!mbar_wait(&v_ready[st], (n_pv / NST) & 1u, abort_flag)) return false;
-                    if (!mbar_wait(p_full, n_pv & 1u, abort_flag)) return false;
+                    if (!mbar_wait_small(&v_ready[st], (n_pv / NST) & 1u, abort_flag)) return false;
+                    if (!mbar_wait_small(p_full, n_pv & 1u, abort_flag)) return false;
                     tcgen05_fence_after();
                     const int steps = load_tile(it, j).chunks * 2;
                     const uint64_t b = dv0 + static_cast<uint64_t>(st * (TILE_BYTES >> 4));
@@ -351,8 +351,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     const WTile tl = load_tile(it, j);
                     const int st = static_cast<int>(t % NST);
                     const uint32_t ph = (t / NST) & 1u;
-                    if (!mbar_wait(&v_full[st], ph, abort_flag)) { ok = false; break; }
-                    if (masked && !mbar_wait(&m_full[st], ph, abort_flag)) { ok = false; break; }
+                    if (!mbar_wait_small(&v_full[st], ph, abort_flag)) { ok = false; break; }
+                    if (masked && !mbar_wait_small(&m_full[st], ph, abort_flag)) { ok = false; break; }
                     __syncwarp();
                     const int there = tl.end - tl.k0;
                     if (masked || there < tl.chunks * 32) {
@@ -389,13 +389,13 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                         mbar_expect_tx(taken, 16);
                         take_over(smem + C::OFF_TAKEN, taken);
                     }
-                    if (!mbar_wait(&id_free[slot], ((n / C::kIds) & 1u) ^ 1u, abort_flag)) break;
+                    if (!mbar_wait_small(&id_free[slot], ((n / C::kIds) & 1u) ^ 1u, abort_flag)) break;
                     WItem it = {};
                     if (id >= 0) it = load_item(p, id);
                     items[slot] = it;
                     mbar_arrive(&id_full[slot]);
                     if (id < 0) break;   // every CTA has started: not asked again
-                    if (!mbar_wait(taken, n & 1u, abort_flag)) break;
+                    if (!mbar_wait_small(taken, n & 1u, abort_flag)) break;
                     id = taken_over(smem + C::OFF_TAKEN);
                 }
             }
@@ -437,8 +437,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     k0 = it.b_lo;
                     end = it.b_hi;
                 }
-                if (masked && !mbar_wait(&m_full[st], (t / NST) & 1u, abort_flag)) { ok = false; break; }
-                if (!mbar_wait(s_full, t & 1u, abort_flag)) { ok = false; break; }
+                if (masked && !mbar_wait_small(&m_full[st], (t / NST) & 1u, abort_flag)) { ok = false; break; }
+                if (!mbar_wait_small(s_full, t & 1u, abort_flag)) { ok = false; break; }
                 __syncwarp();
                 tcgen05_fence_after();
                 // Hidden keys become -inf in TMEM, and so does what lies behind a short tile's last chunk; from there on all kinds
@@ -491,7 +491,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
                 const float alpha = move ? fast_exp2(m_run - m_use) : 1.f;
                 // PV of the item's previous tile is complete: it read the P columns and wrote the accumulator
-                if (j > 0 && !mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
+                if (j > 0 && !mbar_wait_small(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
                 __syncwarp();
                 if (j > 0 && __any_sync(0xffffffffu, move)) {
                     tcgen05_fence_after();
@@ -544,7 +544,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 }
             }
             if (!ok) break;
-            if (!mbar_wait(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
+            if (!mbar_wait_small(o_full, (t - 1u) & 1u, abort_flag)) { ok = false; break; }
             __syncwarp();
             tcgen05_fence_after();
             // The output takes the place of the item's queries (its last QK^T is long done) and leaves by TMA, 32 rows of a warp at
