@@ -1,15 +1,14 @@
 // The 8-bit GEMM of linear_fp8.cu for a few rows (tokens being generated, short requests): bound by the weights' bytes and by
-// latency, not by the tensor pipe, so there is no tile pipeline here.  A CTA owns NT x 8 columns; its W warps share the
-// k-blocks (warp w takes w, w + W, ...), read their part of w and x with 16-byte loads straight into registers, widen the
-// codes to fp16 (exact) and multiply with mma.sync m16n8k16, fp32 accumulation.
-//
-// What it measured: 4096 x 4096, 16 rows: 8.3 us in a graph (weights in L2; from HBM their bytes take 2.6); each warp has two k-blocks in flight
-// (with one: 11.4).
+// latency, not by the tensor pipe, so there is no tile pipeline here.  A CTA owns NT x 8 columns of 8 or 16 rows; its W warps
+// share the k-blocks (warp w takes w, w + W, ...), read their part of w and x with 16-byte loads straight into registers and
+// multiply with mma.sync m16n8k32 (e4m3, fp32 accumulation: 7e-8 from 64 bits).  Each warp has two k-blocks in flight.
+// 16 x 4096 x 4096: 5.8 us in a graph, weights in L2 (from HBM their bytes take 2.6); 11.4 with one k-block in flight and the codes
+// widened to fp16 for m16n8k16, 8.3 with two.
 //
 // No shuffling of operands: a product sums over k in any order as long as both sides agree, so lane (r = lane / 4, c = lane % 4)
 // holds the 16 consecutive codes 16 c .. 16 c + 15 of a 64-wide chunk for weight row r and for x rows r and r + 8, and each of
-// four MMAs takes four codes of a lane.  A k-block's sum is scaled and added to the warp's fp32 sums; the warps' sums meet in shared
-// memory, in the order of the warps.
+// two MMAs takes eight codes of a lane.  A k-block's sum is scaled and added to the warp's fp32 sums; the warps' sums meet in
+// shared memory, in the order of the warps.
 //
 // e4m3 output: a scale block is 128 columns, 8 CTAs' worth of 16.  They form a cluster and exchange their rows' largest
 // magnitudes through distributed shared memory.
@@ -35,12 +34,8 @@ struct RowsParams {
     int out_dtype, res_dtype, epilogue;
 };
 
-__device__ __forceinline__ uint32_t widen2(uint32_t two_codes) {   // two e4m3 codes -> two fp16 values, exactly
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two_codes), __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr, uint32_t rank) {
@@ -103,14 +98,13 @@ __global__ void __launch_bounds__(32 * W, 16 / W) linear_fp8_rows_kernel(const R
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {                      // four codes of each lane
-                auto word = [&](const uint4& v) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); };
-                const uint32_t lo = word(q.x[h][0]), hi = word(q.x[h][XR - 1]);
-                const uint32_t a0 = widen2(lo & 0xFFFFu), a2 = widen2(lo >> 16);
-                const uint32_t a1 = XR == 2 ? widen2(hi & 0xFFFFu) : 0u, a3 = XR == 2 ? widen2(hi >> 16) : 0u;
+            for (int i = 0; i < 2; ++i) {                      // eight codes of each lane
+                const uint4 &lo = q.x[h][0], &hi = q.x[h][XR - 1];
+                const uint32_t a0 = i == 0 ? lo.x : lo.z, a2 = i == 0 ? lo.y : lo.w;
+                const uint32_t a1 = XR == 2 ? (i == 0 ? hi.x : hi.z) : 0u, a3 = XR == 2 ? (i == 0 ? hi.y : hi.w) : 0u;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    mma_f16(part[n], a0, a1, a2, a3, widen2(word(q.w[h][n]) & 0xFFFFu), widen2(word(q.w[h][n]) >> 16));
+                    mma_e4m3(part[n], a0, a1, a2, a3, i == 0 ? q.w[h][n].x : q.w[h][n].z, i == 0 ? q.w[h][n].y : q.w[h][n].w);
             }
         }
 #pragma unroll
@@ -235,26 +229,26 @@ int launch_tiles(const RowsParams& p, int sms, cudaStream_t stream) {
     if (p.out_dtype == B200_E4M3) return launch_rows<XR, 2, 8, true>(p, stream);
     // 8 columns per CTA while that does not make more CTAs than SMs: the more SMs fetch weights at once, the shorter each one's
     // share; sixteen warps where there are k-blocks for more than eight and an SM has but one CTA.
-    const bool narrow = (p.N + 7) / 8 <= sms;
-    if (p.k_blocks > 8 && (narrow || (p.N + 15) / 16 <= sms))
+    const long long down = (p.M + XR * 8 - 1) / (XR * 8);
+    const bool narrow = (p.N + 7) / 8 * down <= sms;
+    if (p.k_blocks > 8 && (narrow || (p.N + 15) / 16 * down <= sms))
         return narrow ? launch_rows<XR, 1, 16, false>(p, stream) : launch_rows<XR, 2, 16, false>(p, stream);
     return narrow ? launch_rows<XR, 1, 8, false>(p, stream) : launch_rows<XR, 2, 8, false>(p, stream);
 }
 
 }  // namespace
 
-// The kernel above pays while its CTAs, 16 rows by 16 columns, fit on the GPU at once, two per SM; clusters of 8 pack less densely.
-// Beyond, tiles read x and w less often.  us per call in a graph, this kernel | tiles, N x K (half-precision linear: 3.2 at the
-// first, 8.4 at the last):
-//   half output  2304 x 768:  M 1 2.5 | 4.5   M 32 3.4 | 4.6   M 64 5.4 | 4.7        1024 x 4096: M 16 4.1 | 12.1  M 48 10.4 | 12.2
-//                4096 x 1024: M 16 3.4 | 5.2  M 24 5.5 | 5.2                         4096 x 4096: M 16 8.3 | 12.4  M 24 14.4 | 12.4
-//   e4m3 output  2304 x 768:  M 16 4.3 | 6.1  M 32 6.4 | 5.9                         4096 x 1024: M 16 4.8 | 6.7   M 24 8.0 | 6.8
-// At 1024 x 4096, 64 rows, 256 CTAs: 13.6 | 12.2, so no more than 48 rows.
+// The kernel above pays while its CTAs, 16 rows by 16 columns, are at most 3.5 per SM; with clusters of 8, 1.75.  Beyond, tiles
+// read x and w less often.  us per call in a graph, this kernel | tiles, N x K:
+//   half output  2304 x 768:  M 1 2.3 | 4.5   M 32 2.9 | 4.6   M 64 4.6 | 4.7        1024 x 4096: M 16 3.6 | 12.1   M 64 6.0 | 12.2
+//                4096 x 1024: M 32 4.9 | 5.3  M 48 6.7 | 5.3                         4096 x 4096: M 32 10.7 | 12.4  M 48 14.9 | 12.4
+//   e4m3 output  2304 x 768:  M 16 3.8 | 6.1  M 32 6.6 | 5.9                         4096 x 1024: M 16 4.8 | 6.8    M 24 7.4 | 6.8
+//                2048 x 2048: M 32 5.6 | 9.0  M 48 9.4 | 9.1                         4096 x 4096: M 16 7.4 | 14.2   M 32 13.8 | 14.0
 bool few_rows_pay(const B200LinearFp8Desc& d, int sms) {
     if (d.M > kFewRows) return false;
     const bool f8 = d.out_dtype == B200_E4M3;
     const long long across = f8 ? (d.N + 127) / 128 * 8 : (d.N + 15) / 16;
-    return (d.M + 15) / 16 * across * 4 <= (f8 ? 7ll : 8ll) * sms;
+    return (d.M + 15) / 16 * across * 4 <= (f8 ? 7ll : 14ll) * sms;
 }
 
 int launch_linear_fp8_rows(const B200LinearFp8Desc& d, cudaStream_t stream, int sms) {
