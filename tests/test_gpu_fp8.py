@@ -362,3 +362,19 @@ def test_feed_forward_in_a_captured_graph_and_on_another_stream(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o.view(torch.uint8), v) for o, v in zip(outs, w))
+
+
+def test_rows_beyond_2_31_elements(cuda_device):
+    M, K, tail = 1_100_000, 2048, 300
+    x = torch.empty(M, K, dtype=BF16, device=cuda_device)
+    x[-tail:] = _randn(cuda_device, 1, tail, K).to(BF16)
+    near = x[-tail:].clone()
+    codes, scales = ops.quantize_fp8(x)
+    want, want_scales = ops.quantize_fp8(near)
+    assert torch.equal(codes[-tail:].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[:, -tail:], want_scales)
+    w8, ws = ops.pack_weight_fp8(0.05 * _randn(cuda_device, 2, K, 64))
+    assert torch.equal(ops.linear_fp8(codes, scales, w8, ws)[-tail:], ops.linear_fp8(want, want_scales, w8, ws))
+    g, b = _randn(cuda_device, 3, K), _randn(cuda_device, 4, K)
+    for far, here in zip(ops.add_layernorm_fp8(x, g, b, 1e-5, half=False)[1:], ops.add_layernorm_fp8(near, g, b, 1e-5, half=False)[1:]):
+        far = far[-tail:] if far.dtype == F8 else far[:, -tail:]
+        assert torch.equal(far.view(torch.uint8), here.view(torch.uint8)) if far.dtype == F8 else torch.equal(far, here)

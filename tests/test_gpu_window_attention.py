@@ -306,3 +306,22 @@ def test_empty_calls(cuda_device):
     k = torch.zeros(2, 5, 64, dtype=F16, device=cuda_device)
     assert ops.window_attention(q, k, k, 1).shape == (2, 0, 64)
     assert ops.window_attention(k[:0], k[:0], k[:0], 1).shape == (0, 5, 64)
+
+
+@pytest.mark.parametrize("Sq", [1, 100])
+def test_places_beyond_2_31_elements_of_a_cache(cuda_device, Sq):
+    Sk, first = 4_400_000, 4
+    cache = torch.empty(2, Sk, 256, dtype=F16, device=cuda_device)            # 4.5 GB, keys and values side by side
+    q_start = torch.tensor([Sk - Sq, Sk - Sq - 1000], dtype=torch.int32, device=cuda_device)
+    q = _randn(cuda_device, 1, 2, Sq, 64).half()
+    kv = []
+    for b, p in enumerate(q_start.tolist()):
+        places = torch.cat([torch.arange(first), torch.arange(p - 300, p + Sq)]).to(cuda_device)
+        rows = _randn(cuda_device, 2 + b, len(places), 256).half()
+        cache[b, places] = rows
+        kv.append(rows)
+    out = ops.window_attention(q, cache[..., :64], cache[..., 64:128], 1, window=(300, 0), sinks=first, kv_len=q_start + Sq, q_start=q_start)
+    near = torch.stack(kv)                                                    # the same, with nothing in between
+    starts = torch.full((2,), first + 300, dtype=torch.int32, device=cuda_device)
+    want, bound, _ = reference(q, near[..., :64], near[..., 64:128], 1, 1, (300, 0), first, q_start=starts)
+    check(out, want, bound)
