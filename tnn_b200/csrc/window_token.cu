@@ -6,6 +6,8 @@
 // may see arrive as zeros), multiplies with mma.sync m16n8k16 (a launch of few rows has no tile for the tcgen05 pipe, and this
 // one waits for memory) and keeps its own running maximum, sum and output.  At the end the warps' results are joined in shared
 // memory and the CTAs' through distributed shared memory: one launch, no workspace, a fixed order of summation.
+// One token of each of 32 sequences of 2000 to 16384 keys, window 8192, 16 / 4 heads: 44 us, 0.78 of the measured copy rate; about 5 us
+// of it are launch, first loads and the join.
 #include "window.cuh"
 #include "ptx.cuh"
 
