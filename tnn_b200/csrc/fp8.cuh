@@ -20,6 +20,11 @@ __device__ __forceinline__ float amax_of_bits(uint32_t bits) {
     const uint32_t least = __float_as_uint(kMinAmax);
     return __uint_as_float(bits > least ? bits : least);
 }
+// max(m, |a|, |b|) for m >= 0, a NaN if there is one (0x7FFFFFFF: the largest magnitude as an integer too)
+__device__ __forceinline__ float amax3(float m, float a, float b) {
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
+    return m;
+}
 __device__ __forceinline__ float encode_scale(float amax) { return __fdiv_rn(kMax, amax); }
 __device__ __forceinline__ float decode_scale(float amax) { return __fdiv_rn(amax, kMax); }
 

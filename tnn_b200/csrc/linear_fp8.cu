@@ -313,7 +313,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
             }
 
             // bias, activation, residual: 32 columns in place
-            uint32_t bits = 0;
+            float top = 0.f;
             auto finish = [&](int c, float (&v)[32]) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], v[2 * j], v[2 * j + 1]);
@@ -395,7 +395,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         if (OUT == kOutF8) {
                             // columns at or beyond N are zeros (no weight, no bias, no residual): they do not move the maximum
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) bits = max(bits, fp8::abs_bits(v[j]));
+                            for (int j = 0; j < 32; j += 2) top = fp8::amax3(top, v[j], v[j + 1]);
                         }
 #pragma unroll
                         for (int j = 0; j < 16; ++j) acc[c * 16 + j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
@@ -428,8 +428,9 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         }
                     }
                 } else {
-                    const float amax = fp8::amax_of_bits(bits);
+                    const float amax = fp8::amax_of_bits(fp8::abs_bits(top));
                     const float enc = fp8::encode_scale(amax);
+                    const uint64_t enc2 = pack_f32x2(enc, enc);
                     uint8_t* srow = strips + lane * 128;
                     if (lane == 0) tma_store_wait_read<0>();
                     __syncwarp();
@@ -439,9 +440,9 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             float a0, a1, a2, a3;
-                            unpack_f32x2(acc[g * 8 + e * 2], a0, a1);
-                            unpack_f32x2(acc[g * 8 + e * 2 + 1], a2, a3);
-                            w[e] = fp8::pack4(a0 * enc, a1 * enc, a2 * enc, a3 * enc);
+                            unpack_f32x2(mul_f32x2(acc[g * 8 + e * 2], enc2), a0, a1);
+                            unpack_f32x2(mul_f32x2(acc[g * 8 + e * 2 + 1], enc2), a2, a3);
+                            w[e] = fp8::pack4(a0, a1, a2, a3);
                         }
                         *reinterpret_cast<uint4*>(srow + ((g ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
