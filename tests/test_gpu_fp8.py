@@ -111,7 +111,8 @@ def test_pack_weight(cuda_device, K, N):
 # ---------------------------------------------------------------------------------------------------- LayerNorm
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("resid", [False, True])
-@pytest.mark.parametrize("rows,H", [(1, 768), (9, 16), (333, 1024), (5, 272), (2, 4096), (1201, 144), (65, 2048), (700, 1552)])
+@pytest.mark.parametrize("rows,H", [(1, 768), (9, 16), (333, 1024), (5, 272), (2, 4096), (1201, 144), (65, 2048), (700, 1552), (31, 784), (130, 1040), (67, 2064), (1500, 2096), (19, 3088),
+                                    (7, 512), (4001, 528), (2999, 1280)])
 def test_add_layernorm_fp8(cuda_device, rows, H, resid, dtype):
     x = _randn(cuda_device, rows + H, rows, H).to(dtype)
     r = _randn(cuda_device, rows + H + 1, rows, H).to(dtype) if resid else None

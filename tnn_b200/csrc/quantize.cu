@@ -114,11 +114,12 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(B200QuantizeFp8Desc d
 }
 
 // ---------------------------------------------------------------- (residual +) LayerNorm -> half and e4m3 + scales
-// A warp per row; a lane holds NV groups of 8 consecutive elements (group g of the lane = elements (g * 32 + lane) * 8 ..),
-// so that 16 lanes hold a block of 128 and its largest magnitude is four shuffles away.  The 8-bit result is rounded from
-// the 32-bit one, not from its half-precision copy.  gamma and beta in shared memory, the next row's loads in flight while
-// this one is reduced.  32768 x 768 f16 with a residual: 32 us, 0.83 of the measured copy rate; what remains is the latency of
-// shuffles and shared memory (four CTAs per SM instead of three, at 64 registers, spill: 39 us).
+// G warps per row; a lane holds NV groups of 8 consecutive elements (group g of lane l of warp w = elements
+// ((g * G + w) * 32 + l) * 8 ..), so that 16 lanes hold a block of 128 and its largest magnitude is four shuffles away.  The 8-bit
+// result is rounded from the 32-bit one, not from its half-precision copy.  gamma and beta in shared memory, the next row's loads
+// in flight while this one is reduced.  With a residual 32768 x 768 f16 31.5 us, 0.85 of the measured copy rate; without one, or where a
+// row does not fill its warps' lanes, bound by instructions and the latency of shuffles and shared memory (0.75; 2096 columns 0.53;
+// two rows on their way were slower from 1024 columns on: 31 against 28 us).
 __device__ __forceinline__ void decode8(const uint4& q, int dtype, float (&v)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -129,21 +130,23 @@ __device__ __forceinline__ void decode8(const uint4& q, int dtype, float (&v)[8]
     }
 }
 
-template <int NV, int DT, bool RESID>
+template <int NV, int G, int DT, bool RESID>
 __global__ void __launch_bounds__(256) add_layernorm_fp8_kernel(B200LayerNormFp8Desc d) {
     extern __shared__ float gb[];   // gamma, then beta: group-major, the 8 elements of a lane's group in two float4 planes
-    const int lane = threadIdx.x & 31;
+    __shared__ float part[2][8];    // the warps' sums and sums of squares, where a row has several warps
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % G;
     const int H = static_cast<int>(d.H);
     const int groups = H >> 3;
-    float* beta_s = gb + NV * 256;
+    float* beta_s = gb + NV * G * 256;
     pdl_launch_dependents();
     pdl_wait();   // gamma and beta too may have been written by the kernel in front
-    const long long nwarps = static_cast<long long>(gridDim.x) * 8;
+    const long long step = static_cast<long long>(gridDim.x) * (8 / G);
     uint4 raw[NV], res[RESID ? NV : 1];
     auto fetch = [&](long long row) {
+        if (row >= d.rows) return;
 #pragma unroll
         for (int g = 0; g < NV; ++g) {
-            const int gi = g * 32 + lane;
+            const int gi = (g * G + w) * 32 + lane;
             raw[g] = make_uint4(0, 0, 0, 0);
             if (RESID) res[g] = make_uint4(0, 0, 0, 0);
             if (gi < groups) {
@@ -152,9 +155,22 @@ __global__ void __launch_bounds__(256) add_layernorm_fp8_kernel(B200LayerNormFp8
             }
         }
     };
-    long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (row < d.rows) fetch(row);
-    for (int i = threadIdx.x; i < NV * 256; i += 256) {
+    // the sum over a row's lanes; all of a row's warps come here the same number of times
+    auto row_sum = [&](float v, float* slots) -> float {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (G > 1) {
+            if (lane == 0) slots[warp] = v;
+            asm volatile("barrier.cta.sync %0, %1;" ::"r"(1 + warp / G), "n"(32 * G) : "memory");
+            v = slots[warp - w];
+#pragma unroll
+            for (int i = 1; i < G; ++i) v += slots[warp - w + i];
+        }
+        return v;
+    };
+    long long row = static_cast<long long>(blockIdx.x) * (8 / G) + warp / G;
+    fetch(row);
+    for (int i = threadIdx.x; i < NV * G * 256; i += 256) {
         const int g = i >> 8, r = i & 255, l = r >> 3, e = r & 7;
         const int at = (g * 2 + (e >> 2)) * 128 + l * 4 + (e & 3);   // conflict-free float4 per lane
         gb[at] = i < H ? __ldg(d.gamma + i) : 0.f;
@@ -162,7 +178,7 @@ __global__ void __launch_bounds__(256) add_layernorm_fp8_kernel(B200LayerNormFp8
     }
     __syncthreads();
     const float inv_h = 1.0f / static_cast<float>(H);
-    for (; row < d.rows; row += nwarps) {
+    for (; row < d.rows; row += step) {
         float v[NV][8];
         float sum = 0.f;
 #pragma unroll
@@ -177,31 +193,27 @@ __global__ void __launch_bounds__(256) add_layernorm_fp8_kernel(B200LayerNormFp8
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += v[g][e];
         }
-        if (row + nwarps < d.rows) fetch(row + nwarps);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float mean = sum * inv_h;
+        fetch(row + step);
+        const float mean = row_sum(sum, part[0]) * inv_h;
         float sq = 0.f;
 #pragma unroll
         for (int g = 0; g < NV; ++g)
-            if (g * 32 + lane < groups) {
+            if ((g * G + w) * 32 + lane < groups) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[g][e] -= mean;
                     sq = fmaf(v[g][e], v[g][e], sq);
                 }
             }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        const float rstd = 1.0f / sqrtf(fmaf(sq, inv_h, d.eps));
+        const float rstd = 1.0f / sqrtf(fmaf(row_sum(sq, part[1]), inv_h, d.eps));
 #pragma unroll
         for (int g = 0; g < NV; ++g) {
-            const int gi = g * 32 + lane;
+            const int ch = g * G + w, gi = ch * 32 + lane;
             uint32_t bits = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float4 gm = *reinterpret_cast<const float4*>(gb + (g * 2 + h) * 128 + lane * 4);
-                const float4 bt = *reinterpret_cast<const float4*>(beta_s + (g * 2 + h) * 128 + lane * 4);
+                const float4 gm = *reinterpret_cast<const float4*>(gb + (ch * 2 + h) * 128 + lane * 4);
+                const float4 bt = *reinterpret_cast<const float4*>(beta_s + (ch * 2 + h) * 128 + lane * 4);
                 v[g][h * 4 + 0] = fmaf(v[g][h * 4 + 0] * rstd, gm.x, bt.x);
                 v[g][h * 4 + 1] = fmaf(v[g][h * 4 + 1] * rstd, gm.y, bt.y);
                 v[g][h * 4 + 2] = fmaf(v[g][h * 4 + 2] * rstd, gm.z, bt.z);
@@ -269,21 +281,43 @@ __global__ void __launch_bounds__(256) pack_weight_fp8_kernel(const float* src, 
 
 constexpr int kQuantizeCtas = 3;   // resident CTAs per SM
 
-template <int NV, int DT>
-void launch_layernorm_fp8(unsigned grid, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
-    const size_t smem = static_cast<size_t>(NV) * 256 * 2 * sizeof(float);
-    if (d.residual) launch_kernel(add_layernorm_fp8_kernel<NV, DT, true>, dim3(grid), dim3(256), smem, stream, d);
-    else launch_kernel(add_layernorm_fp8_kernel<NV, DT, false>, dim3(grid), dim3(256), smem, stream, d);
+template <int NV, int G, int DT, bool RESID>
+int launch_layernorm_fp8(int sms, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
+    static PerDeviceOnce once;
+    static std::atomic<int> resident[kMaxDevices];   // CTAs per SM: the grid is what runs at once, every warp walks rows
+    const size_t smem = static_cast<size_t>(NV) * G * 256 * 2 * sizeof(float);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return B200_ERR_LAUNCH;
+    if (!once.ensure(dev, [&]() {
+            int n = 0;
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, add_layernorm_fp8_kernel<NV, G, DT, RESID>, 256, smem) != cudaSuccess || n < 1)
+                return false;
+            resident[dev].store(n, std::memory_order_relaxed);
+            return true;
+        }))
+        return B200_ERR_LAUNCH;
+    const long long ctas = (d.rows * G + 7) / 8, most = static_cast<long long>(sms) * resident[dev].load(std::memory_order_relaxed);
+    launch_kernel(add_layernorm_fp8_kernel<NV, G, DT, RESID>, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), smem, stream, d);
+    count_launch();
+    return check_launch();
 }
 
-template <int DT>
-void choose_layernorm_fp8(int nv, unsigned grid, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
-    if (nv <= 1) launch_layernorm_fp8<1, DT>(grid, stream, d);
-    else if (nv <= 2) launch_layernorm_fp8<2, DT>(grid, stream, d);
-    else if (nv <= 3) launch_layernorm_fp8<3, DT>(grid, stream, d);
-    else if (nv <= 4) launch_layernorm_fp8<4, DT>(grid, stream, d);
-    else if (nv <= 8) launch_layernorm_fp8<8, DT>(grid, stream, d);
-    else launch_layernorm_fp8<16, DT>(grid, stream, d);
+template <int DT, bool RESID>
+int choose_layernorm_fp8(int sms, cudaStream_t stream, const B200LayerNormFp8Desc& d) {
+    // As few warps per row as let a lane hold 24 values at most.  us for 25 million values, without | with a residual: 1024 columns
+    // one warp 27.7 | 33.8, two 27.1 | 32.9; 2048 columns two warps 32.3 | 34.8, four 29.7 | 34.0; 4096 columns four warps
+    // 36.2 | 39.1, eight 32.7 | 37.8; 768 columns one warp 25.5 | 31.4, two 31.2 | 35.2; 1536 two 27.4 | 38.9, four 33.1 | 40.3.
+    // (One warp for every width: 1024 27.7 | 38.1, 2096 64 | 92, 4096 47 | 73.)
+    int G = 1;
+    while (d.H > 768 * G) G *= 2;
+    const int nv = static_cast<int>((d.H + 256 * G - 1) / (256 * G));
+    switch (G) {
+        case 1: return nv <= 1 ? launch_layernorm_fp8<1, 1, DT, RESID>(sms, stream, d)
+                               : (nv <= 2 ? launch_layernorm_fp8<2, 1, DT, RESID>(sms, stream, d) : launch_layernorm_fp8<3, 1, DT, RESID>(sms, stream, d));
+        case 2: return nv <= 2 ? launch_layernorm_fp8<2, 2, DT, RESID>(sms, stream, d) : launch_layernorm_fp8<3, 2, DT, RESID>(sms, stream, d);
+        case 4: return nv <= 2 ? launch_layernorm_fp8<2, 4, DT, RESID>(sms, stream, d) : launch_layernorm_fp8<3, 4, DT, RESID>(sms, stream, d);
+        default: return launch_layernorm_fp8<2, 8, DT, RESID>(sms, stream, d);
+    }
 }
 
 }  // namespace
@@ -329,15 +363,10 @@ int b200_add_layernorm_fp8_fwd(const B200LayerNormFp8Desc* d, b200_stream_t stre
     if (d->rows == 0) return B200_OK;
     const int sms = lin::device_sm_count();
     if (sms <= 0) return B200_ERR_NOT_SM100;
-    const int nv = static_cast<int>((d->H / 8 + 31) / 32);
-    const int per_sm = nv <= 1 ? 6 : (nv <= 4 ? 3 : (nv <= 8 ? 2 : 1));
-    long long ctas = (d->rows + 7) / 8;
-    if (ctas > static_cast<long long>(sms) * per_sm) ctas = static_cast<long long>(sms) * per_sm;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    if (d->dtype == B200_F16) choose_layernorm_fp8<B200_F16>(nv, static_cast<unsigned>(ctas), stream, *d);
-    else choose_layernorm_fp8<B200_BF16>(nv, static_cast<unsigned>(ctas), stream, *d);
-    count_launch();
-    return check_launch();
+    if (d->dtype == B200_F16)
+        return d->residual ? choose_layernorm_fp8<B200_F16, true>(sms, stream, *d) : choose_layernorm_fp8<B200_F16, false>(sms, stream, *d);
+    return d->residual ? choose_layernorm_fp8<B200_BF16, true>(sms, stream, *d) : choose_layernorm_fp8<B200_BF16, false>(sms, stream, *d);
 }
 
 int b200_pack_weight_fp8(const float* w_kn, int64_t K, int64_t N, int64_t ld_src, void* w_nk, int64_t ld_dst, float* w_scale,
