@@ -32,7 +32,7 @@ def _linear(**kw):
     dict(y=264), dict(bias=260), dict(out_dtype=4), dict(out_dtype=-1), dict(epilogue=4), dict(epilogue=capi.EPI_BIAS_RESIDUAL),
     dict(epilogue=capi.EPI_BIAS_RESIDUAL, residual=256, ldr=56), dict(epilogue=capi.EPI_BIAS_RESIDUAL, residual=256, ldr=64, res_dtype=capi.F32),
     dict(out_dtype=capi.E4M3), dict(out_dtype=capi.E4M3, y_scale=256, ld_y_scale=9), dict(out_dtype=capi.E4M3, y_scale=256, ld_y_scale=10, N=56),
-    dict(block_n=192), dict(block_n=-64), dict(block_n=-1, M=65, ld_x_scale=65), dict(block_n=64, out_dtype=capi.E4M3, y_scale=256, ld_y_scale=10)])
+    dict(block_n=192), dict(block_n=-64), dict(block_n=-1, M=129, ld_x_scale=129), dict(block_n=64, out_dtype=capi.E4M3, y_scale=256, ld_y_scale=10)])
 def test_linear_fp8_refuses(kw):
     assert _linear(**kw) == capi.ERR_PARAM
 

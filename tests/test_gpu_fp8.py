@@ -177,7 +177,7 @@ def test_linear_fp8(cuda_device, M, N, K, out):
 
 @pytest.mark.parametrize("epi", ["none", "bias", "gelu", "tanh", "residual"])
 @pytest.mark.parametrize("M,N,K,block_n", [(m, n, k, bn) for m, n, k in ((41, 200, 400), (300, 392, 272), (513, 256, 128)) for bn in (64, 128, 256)] +
-                         [(1, 8, 16, -1), (3, 200, 400, -1), (16, 1400, 2064, -1), (8, 264, 1040, -1), (9, 4000, 1168, -1), (5, 2600, 272, -1), (41, 264, 1040, -1), (17, 2600, 400, -1)])
+                         [(1, 8, 16, -1), (3, 200, 400, -1), (16, 1400, 2064, -1), (8, 264, 1040, -1), (9, 4000, 1168, -1), (5, 2600, 272, -1), (41, 264, 1040, -1), (17, 2600, 400, -1), (128, 264, 400, -1)])
 def test_linear_fp8_epilogues_on_every_tile(cuda_device, M, N, K, epi, block_n):
     x8, xs, w8, ws = _operands(cuda_device, M, N, K, 5)
     bias = None if epi == "none" else 0.1 * _randn(cuda_device, N, N)
@@ -208,7 +208,7 @@ def test_linear_fp8_epilogues_on_every_tile(cuda_device, M, N, K, epi, block_n):
 
 @pytest.mark.parametrize("epi", ["bias", "gelu", "residual"])
 @pytest.mark.parametrize("M,N,K,block_n", [(m, n, k, bn) for m, n, k in ((1, 16, 64), (41, 272, 400), (300, 1040, 256), (129, 128, 144))
-                                           for bn in (0, 128, 256)] + [(2, 144, 1040, -1), (16, 1040, 400, -1), (7, 272, 2064, -1), (33, 272, 400, -1)])
+                                           for bn in (0, 128, 256)] + [(2, 144, 1040, -1), (16, 1040, 400, -1), (7, 272, 2064, -1), (33, 272, 400, -1), (101, 272, 400, -1)])
 def test_linear_fp8_with_an_8_bit_result(cuda_device, M, N, K, epi, block_n):
     x8, xs, w8, ws = _operands(cuda_device, M, N, K, 7)
     bias = 0.1 * _randn(cuda_device, N, N)
@@ -250,17 +250,17 @@ def test_linear_fp8_rows_do_not_depend_on_the_batch_or_the_tile(cuda_device):
     x8, xs, w8, ws = _operands(cuda_device, 700, 520, 656)
     bias = _randn(cuda_device, 1, 520)
     y = ops.linear_fp8(x8, xs, w8, ws, bias, out_dtype=F32)
-    for rows in (slice(3, 70), slice(100, 400)):
+    for rows in (slice(3, 134), slice(100, 400)):
         part = ops.linear_fp8(x8[rows], xs[:, rows].contiguous(), w8, ws, bias, out_dtype=F32)
         assert torch.equal(part, y[rows])
     for bn in (64, 128, 256):
         assert torch.equal(ops.linear_fp8(x8, xs, w8, ws, bias, out_dtype=F32, block_n=bn), y)
-    few = ops.linear_fp8(x8[:64], xs[:, :64].contiguous(), w8, ws, bias, out_dtype=F32)       # a few rows: an order of its own
+    few = ops.linear_fp8(x8[:128], xs[:, :128].contiguous(), w8, ws, bias, out_dtype=F32)       # a few rows: an order of its own
     for rows in (slice(0, 1), slice(5, 12), slice(3, 44)):
         part = ops.linear_fp8(x8[rows], xs[:, rows].contiguous(), w8, ws, bias, out_dtype=F32)
         assert torch.equal(part, few[rows])
     want, size = _product(x8, xs, w8, ws)
-    _check(few, want[:64] + bias.double(), size[:64] + bias.double().abs(), 656, HALF_STEP[F32])
+    _check(few, want[:128] + bias.double(), size[:128] + bias.double().abs(), 656, HALF_STEP[F32])
 
 
 @pytest.mark.parametrize("out", [F16, F32, F8])

@@ -18,7 +18,7 @@
 // share TMEM.  On 256 columns a k-block costs 0.48 us (its UMMAs alone 0.32), a tile 2.6 us beside its k-blocks.
 // 16384 x 4096 x 4096 with an f16 result 293 us (1870 TFLOP/s), K = 1024 101 us, f32 110, e4m3 102 (with GELU 128), GELU 123, residual 133.
 // Pairs of CTAs on 256 x 256 and 256 x 128 tiles took 107 and 113 us at K = 1024, two CTAs per SM on 128 x 128 95 but 157 with GELU.
-// Up to 64 rows linear_fp8_rows.cu does the same without a pipeline.
+// For up to 128 rows and few columns linear_fp8_rows.cu does the same without a pipeline.
 #include "fp8.cuh"
 #include "linear_common.cuh"
 #include "linear_fp8.cuh"

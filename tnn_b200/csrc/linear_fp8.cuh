@@ -5,7 +5,7 @@
 namespace b200 {
 namespace lin {
 
-constexpr int kFewRows = 64;   // the kernel for a few rows takes no more
+constexpr int kFewRows = 128;   // the kernel for a few rows takes no more
 bool few_rows_pay(const B200LinearFp8Desc& d, int sms);
 int launch_linear_fp8_rows(const B200LinearFp8Desc& d, cudaStream_t stream, int sms);
 

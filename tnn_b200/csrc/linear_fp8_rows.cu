@@ -242,6 +242,7 @@ int launch_tiles(const RowsParams& p, int sms, cudaStream_t stream) {
 // read x and w less often.  us per call in a graph, this kernel | tiles, N x K:
 //   half output  2304 x 768:  M 1 2.3 | 4.5   M 32 2.9 | 4.6   M 64 4.6 | 4.7        1024 x 4096: M 16 3.6 | 12.1   M 64 6.0 | 12.2
 //                4096 x 1024: M 32 4.9 | 5.3  M 48 6.7 | 5.3                         4096 x 4096: M 32 10.7 | 12.4  M 48 14.9 | 12.4
+//                1024 x 1024: M 128 4.6 | 5.4  M 160 5.8 | 5.4                      1024 x 4096: M 128 10.7 | 12.4
 //   e4m3 output  2304 x 768:  M 16 3.8 | 6.1  M 32 6.6 | 5.9                         4096 x 1024: M 16 4.8 | 6.8    M 24 7.4 | 6.8
 //                2048 x 2048: M 32 5.6 | 9.0  M 48 9.4 | 9.1                         4096 x 4096: M 16 7.4 | 14.2   M 32 13.8 | 14.0
 bool few_rows_pay(const B200LinearFp8Desc& d, int sms) {
