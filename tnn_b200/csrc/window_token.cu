@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
     const float* mask = MASKED ? p.mask_add + static_cast<long long>(b) * p.Sk : nullptr;
     const uint32_t ring_u = smem_u32(ring);
 
+    // keys that every row of the block sees: the window's between these
+    const int all_lo = p0 + (r0 + rows - 1) / p.group - p.left, all_hi = p0 + r0 / p.group + p.right;
     const int tiles = (n + kTile - 1) / kTile;
     const int first = rank * kWarps + warp, step = ctas * kWarps;
     auto fetch = [&](int tile, int stage) {                // tile's keys and values; beyond the last tile an empty group
@@ -188,30 +190,42 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
         // scale, mask, running maximum
         float alpha[MT][2];
         bool moved = false;
+        const int at0 = tile * kTile;
+        const bool plain = !MASKED && at0 >= n_a && at0 + kTile <= n && at0 + shift >= all_lo && at0 + shift + kTile - 1 <= all_hi;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             float top[2] = {-INFINITY, -INFINITY};
+            if (plain) {                                   // (a row that does not exist goes along: it is not stored)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int at = tile * kTile + j * 8 + c2 + e;
-                    const int key = at + (at >= n_a ? shift : 0);
-                    float mk = 0.f;
-                    bool there = at < n;
-                    if (MASKED) {
-                        mk = there ? mask[key] : 0.f;
-                        there = there && mk > p.mask_below;
-                        mk *= kLog2e;
+                    for (int e = 0; e < 4; ++e) {
+                        s[t][j][e] *= p.scale_log2;
+                        top[e >> 1] = fmaxf(top[e >> 1], s[t][j][e]);
                     }
+            } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const bool seen = there && ((key >= lo[t][h] && key <= hi[t][h]) || key < first_keys[t][h]);
-                        const float x = seen ? fmaf(s[t][j][h * 2 + e], p.scale_log2, mk) : -INFINITY;
-                        s[t][j][h * 2 + e] = x;
-                        top[h] = fmaxf(top[h], x);
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int at = at0 + j * 8 + c2 + e;
+                        const int key = at + (at >= n_a ? shift : 0);
+                        float mk = 0.f;
+                        bool there = at < n;
+                        if (MASKED) {
+                            mk = there ? mask[key] : 0.f;
+                            there = there && mk > p.mask_below;
+                            mk *= kLog2e;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const bool seen = there && ((key >= lo[t][h] && key <= hi[t][h]) || key < first_keys[t][h]);
+                            const float x = seen ? fmaf(s[t][j][h * 2 + e], p.scale_log2, mk) : -INFINITY;
+                            s[t][j][h * 2 + e] = x;
+                            top[h] = fmaxf(top[h], x);
+                        }
                     }
-                }
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
