@@ -6,8 +6,8 @@
 // may see arrive as zeros), multiplies with mma.sync m16n8k16 (a launch of few rows has no tile for the tcgen05 pipe, and this
 // one waits for memory) and keeps its own running maximum, sum and output.  At the end the warps' results are joined in shared
 // memory and the CTAs' through distributed shared memory: one launch, no workspace, a fixed order of summation.
-// One token of each of 32 sequences of 2000 to 16384 keys, window 8192, 16 / 4 heads: 44 us, 0.78 of the measured copy rate; about 5 us
-// of it are launch, first loads and the join.
+// One token of each of 32 sequences of 2000 to 16384 keys, window 8192, 16 / 4 heads: 43 us, 0.80 of the measured copy rate (0.96 where
+// all have 16384); about 5 us of it are launch, first loads and the join.
 #include "window.cuh"
 #include "ptx.cuh"
 
@@ -414,14 +414,23 @@ bool token_kernel_takes(const WindowParams& p) {
 }
 
 int launch_window_token(const WindowParams& p, int dtype, int sms, cudaStream_t stream) {
-    // As many CTAs per key / value head as one wave of two per SM holds, each with a tile for every warp at least.  (32 sequences,
-    // 4 key / value heads, window 8192: 2 CTAs each 44.6 us, 4 (1.7 waves) 48.5, 8 56.4.)
+    // The number of CTAs per key / value head with the smallest waves x (fixed cost + keys of a CTA), two CTAs per SM; a CTA's start
+    // and join cost as much as some 600 keys (5.5 us).  us on 1 | 2 | 4 | 8: 32 sequences, 4 heads, window 8192 54.7 | 43.0 | 46.1 | 55.1;
+    // 27 of 6088 keys, 12 heads 103 | 90 | 88 | 101; 60 of 5575, 4 heads, 5 tokens 64 | 71 | 84 | 111; 8 of 5711, 12 heads
+    // 37.3 | 25.7 | 31.6 | 32.5; 4 of 4096, 8 heads 21.7 | 14.6 | 10.3 | 7.9.
     const int blocks = (p.Sq * p.group + kBlockRows - 1) / kBlockRows;
     const long long units = static_cast<long long>(p.B) * (p.heads / p.group) * blocks;
     const long long reach = static_cast<long long>(p.left) + p.right + p.Sq + p.sinks;
     const long long keys = p.Sk < reach ? p.Sk : reach;
     int ctas = 1;
-    while (ctas < 8 && units * ctas * 2 <= 2ll * sms && keys >= 2ll * ctas * kWarps * kTile) ctas *= 2;
+    long long least = 0;
+    for (int c = 1; c <= 8 && (c == 1 || keys >= static_cast<long long>(c) * kWarps * kTile); c *= 2) {   // a tile for every warp
+        const long long t = (units * c + 2 * sms - 1) / (2 * sms) * (600 + keys / c);
+        if (c == 1 || t < least) {
+            least = t;
+            ctas = c;
+        }
+    }
     if (p.mask_add != nullptr)
         return dtype == B200_F16 ? launch_rows<B200_F16, true>(p, ctas, blocks, stream) : launch_rows<B200_BF16, true>(p, ctas, blocks, stream);
     return dtype == B200_F16 ? launch_rows<B200_F16, false>(p, ctas, blocks, stream) : launch_rows<B200_BF16, false>(p, ctas, blocks, stream);
