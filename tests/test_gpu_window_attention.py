@@ -95,6 +95,24 @@ def test_self_attention_windows(cuda_device, S, window, sinks, dtype):
     run(cuda_device, 2, S, S, 2, 2, window, sinks, dtype, seed=S)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("window,sinks", [((142, 142), 16), ((6, 6), 1), ((2, 2), 40), ((30, 3), 70), ((17, 0), 96), ((100, 60), 33), ((0, 31), 97), ((3, 0), 95)])
+def test_first_tokens_behind_a_short_last_tile(cuda_device, window, sinks, masked, dtype):
+    mask = None
+    if masked:
+        mask = torch.zeros(3, 700, device=cuda_device)
+        mask[:, [1, 30, 31, 32, 69, 500]] = -10000.0
+        mask[:, 0], mask[:, 2::7] = 1.5, -2.0
+    q, k, v, kv_len, _, out = run(cuda_device, 3, 700, 700, 2, 1, window, sinks, dtype, lens=[700, 433, 20], mask=mask, seed=sinks)
+    # at the end of a cache: places between the first tokens and the windows may hold anything
+    starts = torch.tensor([500, 400, 300], dtype=torch.int32, device=cuda_device)
+    clean = ops.window_attention(q[:, :150], k, v, 2, 1, window=window, sinks=sinks, q_start=starts, mask_add=mask)
+    k, v = k.clone(), v.clone()
+    k[:, sinks:300 - window[0]], v[:, sinks:300 - window[0]] = math.nan, math.inf
+    assert torch.equal(ops.window_attention(q[:, :150], k, v, 2, 1, window=window, sinks=sinks, q_start=starts, mask_add=mask), clean)
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(4, 4), (4, 2), (4, 1), (6, 3)])
 @pytest.mark.parametrize("window,sinks", [((100, 100), 2), ((50, 0), 0)])
 def test_grouped_heads_and_ragged_lengths(cuda_device, heads, kv_heads, window, sinks):

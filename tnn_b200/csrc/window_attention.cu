@@ -4,16 +4,17 @@
 // The keys that a block of 128 queries can see are at most two runs: the first tokens [0, sinks) and the window
 // [p_first - left, p_last + right], one run where they touch.  An item (128 queries of one head of one sequence) walks the
 // runs in tiles of up to 128 keys that start where the run starts, not at multiples of 128; the last tile of a run is as
-// short as the run needs, in steps of 32 keys (QK^T with N = 32 c, PV with K = 32 c, c chunks of softmax), so that four sinks
-// cost a quarter of a tile.
+// short as the run needs, in steps of 32 keys (QK^T with N = 32 c, PV with K = 32 c, c chunks of softmax).  First tokens that fit
+// behind the window's last, short tile share it; otherwise they have a tile of their own, four sinks a quarter of one.
 //
 // tcgen05 (S = Q K^T, O += P V), one softmax warpgroup, online softmax with lazy maximum; two CTAs per SM, so that one's exp
 // pass covers the other's hand-offs.  How long an item takes depends on its sequence's length and on its place in it, so items
 // are not dealt in advance: the grid has a CTA per item, and a running CTA takes over the next one that has not started
 // (cluster launch control), prefetching its queries and scores while it is still at work on its own.
 //
-// 16384 causal queries, window 1024, 4 sinks, 16 / 4 heads, bf16: 139 us (67 GFLOP visible; the exp unit's floor is 58), 4 x 4096 queries,
-// window 256 to both sides, ragged: 63 to 67 us.  The exp unit is 56 % busy: the two softmax warps of a scheduler wait for fixed
+// 16384 causal queries, window 1024, 4 sinks, 16 / 4 heads, bf16: 142 us (67 GFLOP visible; the exp unit's floor is 58), 4 x 4096 queries,
+// window 256 to both sides, ragged: 59 to 67 us.  First tokens that share a tile: 11 x 1302 queries, window 142 to both sides, 16 sinks
+// 69 -> 64 us, 16 x 393, window 6, 28 -> 24.7; windows of whole tiles pay up to 2 % for it (139.6 -> 142).  The exp unit is 56 % busy: the two softmax warps of a scheduler wait for fixed
 // latencies and tend to be in the exp pass together.  Exponentials by a polynomial (1/4 of them 153 us), two threads per row
 // (140), both passes rolled (155) did not help.
 #include "linear_common.cuh"
@@ -27,6 +28,7 @@ namespace {
 constexpr int TQ = 128;                      // queries per item
 constexpr int TK = 128;                      // keys per tile at most
 constexpr int TILE_BYTES = 128 * HD * 2;
+constexpr int CHUNK_BYTES = 32 * HD * 2;     // a load: 32 keys
 constexpr float kLazyLog2 = 8.0f;            // the running maximum moves only when a tile exceeds it by more than 2^8
 
 struct TileParams : WindowParams {
@@ -46,7 +48,7 @@ struct TileParams : WindowParams {
 // TMEM: S 128 columns, O 64, P 64 (half precision, the A operand of PV).
 struct WCfg {
     static constexpr int THREADS = 256;
-    static constexpr int REGS_CONTROL = 64, REGS_SOFTMAX = 192;
+    static constexpr int REGS_CONTROL = 72, REGS_SOFTMAX = 184;
     static constexpr int NST = 2;
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_K = 2 * TILE_BYTES;
@@ -66,8 +68,9 @@ static_assert(128 * WCfg::REGS_CONTROL + 128 * WCfg::REGS_SOFTMAX <= 65536 / 2, 
 struct __align__(16) WItem {
     int b, head, q0, p0;      // p0: position of the item's first query
     int a_end, b_lo, b_hi;    // the runs
-    int there;                // 0: no further item
-    __device__ __forceinline__ int tiles_a() const { return (a_end + TK - 1) / TK; }
+    int there;                // 0: no further item; 1 + the chunks of the first tokens that share the last tile
+    __device__ __forceinline__ int shared() const { return there - 1; }
+    __device__ __forceinline__ int tiles_a() const { return there > 1 ? 0 : (a_end + TK - 1) / TK; }
     __device__ __forceinline__ int tiles() const { return tiles_a() + (b_hi - b_lo + TK - 1) / TK; }
 };
 
@@ -93,7 +96,9 @@ __device__ __forceinline__ int taken_over(const void* answer) {
     return ok ? static_cast<int>(x) : -1;
 }
 struct WTile {
-    int k0, end, chunks;      // first key, end of its run, 32-key chunks
+    int k0, end, own, chunks; // first key, end of its run, 32-key chunks of the run and all (the first tokens' behind them)
+    __device__ __forceinline__ int first(int c) const { return c < own ? k0 + c * 32 : (c - own) * 32; }   // key of chunk c
+    __device__ __forceinline__ int limit(int c, const WItem& it) const { return c < own ? end : (c < chunks ? it.a_end : 0); }
 };
 
 __device__ __forceinline__ WItem load_item(const TileParams& p, int id) {
@@ -109,6 +114,8 @@ __device__ __forceinline__ WItem load_item(const TileParams& p, int id) {
     it.b_lo = r.b_lo;
     it.b_hi = r.b_hi;
     it.there = 1;
+    const int tiles_b = (r.b_hi - r.b_lo + TK - 1) / TK, a = (r.a_end + 31) >> 5;
+    if (a > 0 && tiles_b > 0 && a + ((r.b_hi - r.b_lo - (tiles_b - 1) * TK + 31) >> 5) <= TK / 32) it.there = 1 + a;
     return it;
 }
 __device__ __forceinline__ WTile load_tile(const WItem& it, int j) {
@@ -116,7 +123,8 @@ __device__ __forceinline__ WTile load_tile(const WItem& it, int j) {
     const int n_a = it.tiles_a();
     t.k0 = j < n_a ? j * TK : it.b_lo + (j - n_a) * TK;
     t.end = j < n_a ? it.a_end : it.b_hi;
-    t.chunks = (min(TK, t.end - t.k0) + 31) >> 5;
+    t.own = (min(TK, t.end - t.k0) + 31) >> 5;
+    t.chunks = t.own + (j == it.tiles() - 1 ? it.shared() : 0);
     return t;
 }
 
@@ -235,27 +243,28 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     tma_load_3d(smem + C::OFF_Q + set * TILE_BYTES, &tm_q, &q_full[set], it.head * HD, it.q0, it.b);
                 }
                 ++k;
+#pragma unroll 1
                 for (int j = 0; j < n_tiles; ++j, ++t) {
                     const WTile tl = load_tile(it, j);
                     const int st = static_cast<int>(t % NST);
                     const uint32_t ph = ((t / NST) & 1u) ^ 1u;
                     if (!mbar_wait_small(&k_empty[st], ph, abort_flag)) { ok = false; break; }
-                    if (lane == 0) {
-                        mbar_expect_tx(&k_full[st], TILE_BYTES);
-                        tma_load_3d(smem + C::OFF_K + st * TILE_BYTES, &tm_k, &k_full[st], kv_col, tl.k0, it.b);
-                    }
+                    if (lane == 0) mbar_expect_tx(&k_full[st], tl.chunks * CHUNK_BYTES);
+                    __syncwarp();
+                    if (lane < tl.chunks)
+                        tma_load_3d(smem + C::OFF_K + st * TILE_BYTES + lane * CHUNK_BYTES, &tm_k, &k_full[st], kv_col, tl.first(lane), it.b);
                     if (!mbar_wait_small(&v_empty[st], ph, abort_flag)) { ok = false; break; }   // also: the stage's mask is done with
-                    if (lane == 0) {
-                        mbar_expect_tx(&v_full[st], TILE_BYTES);
-                        tma_load_3d(smem + C::OFF_V + st * TILE_BYTES, &tm_v, &v_full[st], kv_col, tl.k0, it.b);
-                    }
+                    if (lane == 0) mbar_expect_tx(&v_full[st], tl.chunks * CHUNK_BYTES);
+                    __syncwarp();
+                    if (lane < tl.chunks)
+                        tma_load_3d(smem + C::OFF_V + st * TILE_BYTES + lane * CHUNK_BYTES, &tm_v, &v_full[st], kv_col, tl.first(lane), it.b);
                     if (masked) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            const int key = tl.k0 + c * 32 + lane;
+                            const int key = tl.first(c) + lane;
                             float m = 0.f;
                             bool seen = false;
-                            if (key < tl.end && p.mask_add != nullptr) {
+                            if (key < tl.limit(c, it) && p.mask_add != nullptr) {
                                 m = p.mask_add[static_cast<long long>(it.b) * p.Sk + key];
                                 seen = m > p.mask_below;
                             }
@@ -302,6 +311,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     tcgen05_fence_after();
                     const int steps = load_tile(it, j).chunks * 2;
                     const uint64_t b = dv0 + static_cast<uint64_t>(st * (TILE_BYTES >> 4));
+#pragma unroll 2
                     for (int e = 0; e < steps; ++e)   // P: 8 columns per 16 keys, V: 2 KB per 16 keys
                         umma_f16_ts(tmem_base + C::COL_O, tmem_base + C::COL_P + e * 8, b + static_cast<uint64_t>(e * (2048 >> 4)),
                                     p.idesc_pv, (j | e) != 0 ? 1u : 0u);
@@ -359,11 +369,11 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     if (!mbar_wait_small(&v_full[st], ph, abort_flag)) { ok = false; break; }
                     if (masked && !mbar_wait_small(&m_full[st], ph, abort_flag)) { ok = false; break; }
                     __syncwarp();
-                    const int there = tl.end - tl.k0;
-                    if (masked || there < tl.chunks * 32) {
+                    if (masked || tl.end - tl.k0 < tl.own * 32 || tl.own < tl.chunks) {
                         uint8_t* v = smem + C::OFF_V + st * TILE_BYTES;
+#pragma unroll 1
                         for (int c = 0; c < tl.chunks; ++c) {
-                            uint32_t hide = ~low_bits(there - c * 32);
+                            uint32_t hide = ~low_bits(tl.limit(c, it) - tl.first(c));
                             if (masked) hide |= ~bits_s[st * 4 + c];
                             while (hide != 0) {   // four rows of 128 bytes at a time, 8 lanes each (zeros need no swizzle)
                                 uint32_t rest = hide;
@@ -421,6 +431,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 const int q = it.q0 + r_in_tile;
                 uint16_t* dst = static_cast<uint16_t*>(p.out) + it.b * p.o_batch + q * p.ldo + it.head * HD;
                 if (q < p.Sq)
+#pragma unroll 1
                     for (int g = 0; g < HD / 8; ++g) *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(0, 0, 0, 0);
                 continue;
             }
@@ -434,7 +445,8 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             const int row_lo = it.p0 + r_in_tile - p.left, row_hi = it.p0 + r_in_tile + p.right;
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n_tiles; ++j, ++t) {
-                const WTile tl = {k0, end, (min(TK, end - k0) + 31) >> 5};
+                const int own = (min(TK, end - k0) + 31) >> 5, with = j + 1 == n_tiles ? it.shared() : 0, chunks = own + with;
+                int first = k0, limit = end;   // of the chunk at hand, behind the run's own the first tokens'
                 const int st = static_cast<int>(t % NST);
                 const bool plain = j < plain_a || (j >= plain_lo && j < plain_hi);
                 k0 += TK;
@@ -449,14 +461,18 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 // Hidden keys become -inf in TMEM, and so does what lies behind a short tile's last chunk; from there on all kinds
                 // of tiles share one path.  What bounds this kernel first is fetching instructions: with the edges' code in the
                 // passes below, unrolled four times over, and unrolled waits it was 69 KB long and took 150 us for 16384 causal
-                // queries of 16 heads, window 1024; 49 KB take 139.6.
+                // queries of 16 heads, window 1024; 49 KB took 139.6.
                 if (!plain) {
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t s[32];
-                        const int first = tl.k0 + c * 32;
                         uint32_t bits = (low_bits(row_hi + 1 - first) & ~low_bits(row_lo - first)) | low_bits(p.sinks - first);
-                        bits &= low_bits(tl.end - first);
+                        bits &= low_bits(limit - first);
+                        first += 32;
+                        if (c + 1 == own) {
+                            first = 0;
+                            limit = with != 0 ? it.a_end : 0;
+                        }
                         tmem_ld_32x32b_x32(t_s + c * 32, s);
                         tmem_ld_wait(s);
                         if (masked) {
@@ -515,7 +531,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 uint64_t ps2[2] = {0ull, 0ull};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    if (c < tl.chunks) {
+                    if (c < chunks) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
@@ -685,8 +701,8 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     const uint64_t os[2] = {static_cast<uint64_t>(d->ldo) * 2, static_cast<uint64_t>(p.o_batch) * 2};
     const uint32_t strip[3] = {HD, 32, 1};
     CUtensorMap tq, tk, tv, to;
-    if (!get_tensor_map(&tq, d->q, 3, qd, qs, box) || !get_tensor_map(&tk, d->k, 3, kd, ks, box) ||
-        !get_tensor_map(&tv, d->v, 3, kd, vs, box) || !get_tensor_map(&to, d->out, 3, qd, os, strip))
+    if (!get_tensor_map(&tq, d->q, 3, qd, qs, box) || !get_tensor_map(&tk, d->k, 3, kd, ks, strip) ||
+        !get_tensor_map(&tv, d->v, 3, kd, vs, strip) || !get_tensor_map(&to, d->out, 3, qd, os, strip))
         return B200_ERR_DRIVER;
     if (!set_window_attributes(dev)) return B200_ERR_LAUNCH;
     const dim3 grid(static_cast<unsigned>(items));
