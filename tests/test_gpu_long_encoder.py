@@ -147,3 +147,48 @@ def test_refusals(cuda_device):
     for kw in ({"fp8": True}, {"window": (4, 4)}):
         with pytest.raises(ValueError):
             Encoder.from_workload(wl, torch.float16, cuda_device, fold_layernorm=True, **kw)
+
+
+def test_calls_at_once_on_several_streams_and_in_graphs(cuda_device):
+    def randn(seed, *shape):
+        return torch.randn(*shape, generator=torch.Generator(device="cpu").manual_seed(seed)).to(cuda_device)
+
+    def attention(B, S, heads, kv_heads, window, sinks, Sq):
+        q, k, v = (randn(i, B, n, h * 64).half() for i, n, h in ((1, Sq, heads), (2, S, kv_heads), (3, S, kv_heads)))
+        start = torch.full((B,), S - Sq, dtype=torch.int32, device=cuda_device)
+        return lambda: ops.window_attention(q, k, v, heads, kv_heads, window=window, sinks=sinks, q_start=start)
+
+    def linear(M, N, K, out):
+        x8, xs = ops.quantize_fp8(randn(4, M, K))
+        w8, ws = ops.pack_weight_fp8(0.05 * randn(5, K, N))
+        y = lambda: ops.linear_fp8(x8, xs, w8, ws, epilogue=ops.EPI_BIAS_GELU, out_dtype=out)   # noqa: E731
+        return (lambda: y()[0].view(torch.uint8)) if out == F8 else y
+
+    def norm(M, H):
+        x, g, b = randn(6, M, H).half(), randn(7, H), randn(8, H)
+        return lambda: ops.add_layernorm_fp8(x, g, b, 1e-5, residual=x)[0]
+
+    jobs = [attention(3, 1500, 8, 2, (200, 0), 4, 1500), attention(40, 300, 4, 4, (20, 20), 1, 300), attention(7, 3000, 16, 4, (-1, 0), 0, 1),
+            linear(2000, 1024, 1024, torch.float16), linear(5, 2304, 768, torch.float16), linear(100, 1024, 512, F8),
+            linear(2000, 1024, 512, F8), norm(2000, 2096), norm(500, 768), norm(1000, 4096)]
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(10):
+        got = []
+        for job, stream in zip(jobs, streams):
+            with torch.cuda.stream(stream):
+                got.append([job() for _ in range(3)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+    graphs = []
+    for job in jobs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, [job() for _ in range(3)]))
+    for _ in range(10):
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for (_, ys), w in zip(graphs, want) for y in ys)
