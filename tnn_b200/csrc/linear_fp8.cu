@@ -562,20 +562,21 @@ int validate_linear_fp8(const B200LinearFp8Desc* d) {
     return B200_OK;
 }
 
-// The tile of the smallest estimated time: waves of tiles over the SMs x (per tile + per k-block), in us, fitted to one and two
-// waves measured in a CUDA graph.  us per launch on 64 | 128 | 256 columns:  41 rows 768 -> 2304 4.5 | 5.1 | 7.2;  777 rows
-// 768 -> 2304 7.5 | 6.0 | 8.0, 1024 -> 1024 5.6 | 6.4 | 8.8, 1024 -> 4096 13.7 | 10.5 | 9.5;  1300 rows 1024 -> 1024 8.2 | 6.6 | 8.9,
-// 4096 -> 1024 22.1 | 15.2 | 21.2;  4096 rows 1024 -> 1024 14.4 | 10.8 | 9.4;  8192 rows 1024 -> 4096 81 | 57 | 49.
+// The tile of the smallest estimated time: waves of tiles over the SMs x (per tile + per k-block) + what the last tile's epilogue
+// adds, in us, fitted to launches measured in a CUDA graph; over 60 drawn shapes the choice costs 0.2 % more than the best.
+// us per launch on 64 | 128 | 256 columns:  777 rows 768 -> 2304 7.5 | 6.0 | 8.0, 1024 -> 1024 5.6 | 6.4 | 8.8, 1024 -> 4096
+// 13.7 | 10.5 | 9.5;  1300 rows 1024 -> 1024 8.2 | 6.6 | 8.9, 4096 -> 1024 22.1 | 15.2 | 21.2;  4096 rows 1024 -> 1024
+// 14.4 | 10.8 | 9.4;  8192 rows 1024 -> 4096 81 | 57 | 49;  41339 rows 480 -> 832 59.8 | 39.9 | 45.2.
 int choose_columns(const B200LinearFp8Desc& d, int sms) {
     const bool f8 = d.out_dtype == B200_E4M3;   // no 64-wide form; 128-wide tiles have half the epilogue warps
     const int columns[3] = {64, 128, 256};
-    const double per_tile[3] = {0.73, f8 ? 2.4 : 1.6, 2.6}, per_block[3] = {0.29, f8 ? 0.40 : 0.31, 0.484};
+    const double per_tile[3] = {0.73, f8 ? 1.8 : 1.25, 2.6}, per_block[3] = {0.29, f8 ? 0.335 : 0.31, 0.484}, last[3] = {0.0, f8 ? 0.6 : 0.4, 0.0};
     const double k_blocks = static_cast<double>((d.K + 127) / 128);
     int best = 256;
     double best_t = 1e300;
     for (int i = f8 ? 1 : 0; i < 3; ++i) {
         const int64_t tiles = (d.M + 127) / 128 * ((d.N + columns[i] - 1) / columns[i]);
-        const double t = static_cast<double>((tiles + sms - 1) / sms) * (per_tile[i] + per_block[i] * k_blocks);
+        const double t = static_cast<double>((tiles + sms - 1) / sms) * (per_tile[i] + per_block[i] * k_blocks) + last[i];
         if (t < best_t) {
             best_t = t;
             best = columns[i];
