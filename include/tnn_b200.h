@@ -372,7 +372,7 @@ B200_API int b200_linear_fp8_fwd(const B200LinearFp8Desc* desc, b200_stream_t st
  *   sinks       : how many first keys every query sees (0 = none).
  *   kv_len      : int32 [B], keys of each sequence (clamped to Sk; <= 0: none), or NULL (= Sk).
  *   q_start     : int32 [B], position of each sequence's first query, or NULL (= 0): Sq new tokens at the end of a cache
- *                 of kv_len keys have q_start = kv_len - Sq.
+ *                 of kv_len keys have q_start = kv_len - Sq.  Any value, beside any left and right: positions are 64-bit.
  *   mask_add    : fp32 [B, Sk] additive key mask or NULL.  A key whose value is <= mask_exclude_below, <= -2^127 or
  *                 NaN is dropped.
  *   A query that sees no key yields a row of zeros.  K and V rows that no query of the sequence may see (outside every query's

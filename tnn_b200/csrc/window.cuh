@@ -24,24 +24,41 @@ struct WindowParams {
     const void* v;
     int Sq, Sk, heads, group;           // group = heads / kv_heads
     long long ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch;
-    int left, right;                    // both clamped to kUnlimited where there is no limit
+    long long left, right;              // >= 0, kUnlimited where there is no limit
     int sinks;
     float scale_log2, mask_below;
     int B;
     unsigned int* status;
 };
 constexpr float kLeastMask = -1.7014118e38f;  // -2^127: a mask at or below it is dropped whatever the threshold (x log2(e) it must stay finite)
-constexpr int kUnlimited = 1 << 28;          // beyond every position (Sq, Sk <= 2^24, q_start clamped to +-2^26)
+constexpr long long kUnlimited = 1ll << 40;  // reaches every key from every 32-bit position
 
-// The keys that queries at positions [p_first, p_last] of a sequence can see, as runs [0, a_end) and [b_lo, b_hi).
+// The window of a sequence's first query, [lo, hi]; query i has [lo + i, hi + i].  The sums are taken in 64 bits and clamped to
+// +-2^25, which changes nothing that is visible: keys and i are below 2^24, so beyond the clamp every key lies on the same side
+// of the limit for every query.  (A clamped position with an unclamped width next to it would not do: position 2^27 and a window
+// of 2^26 to the left see nothing.)
+struct Window {
+    int lo, hi;
+};
+__device__ __forceinline__ Window first_window(const WindowParams& p, int b) {
+    const long long pos = p.q_start == nullptr ? 0 : p.q_start[b];
+    constexpr long long kEnd = 1ll << 25;
+    Window w;
+    w.lo = static_cast<int>(min(max(pos - p.left, -kEnd), kEnd));
+    w.hi = static_cast<int>(min(max(pos + p.right, -kEnd), kEnd));
+    return w;
+}
+
+// The keys that a run of queries of a sequence can see, as runs [0, a_end) and [b_lo, b_hi); `lo` is where the first one's window
+// begins, `hi` where the last one's ends.
 struct Runs {
     int a_end, b_lo, b_hi;
 };
-__device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int p_first, int p_last) {
+__device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int lo, int hi) {
     Runs r;
     r.a_end = min(p.sinks, kv);
-    r.b_lo = max(0, p_first - p.left);
-    r.b_hi = min(kv, p_last + p.right + 1);
+    r.b_lo = max(0, lo);
+    r.b_hi = min(kv, hi + 1);
     if (r.b_hi <= r.b_lo) {                  // nothing but the first tokens
         r.b_lo = r.b_hi = 0;
     } else if (r.b_lo <= r.a_end) {          // the runs touch
@@ -54,10 +71,6 @@ __device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int 
 __device__ __forceinline__ int sequence_keys(const WindowParams& p, int b) {
     if (p.kv_len == nullptr) return p.Sk;
     return min(max(p.kv_len[b], 0), p.Sk);
-}
-__device__ __forceinline__ int first_position(const WindowParams& p, int b) {
-    if (p.q_start == nullptr) return 0;
-    return min(max(p.q_start[b], -(1 << 26)), 1 << 26);
 }
 // bits [0, n) of a word, n clamped to [0, 32]
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }

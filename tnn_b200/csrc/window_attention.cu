@@ -57,8 +57,8 @@ struct WCfg {
     static constexpr int OFF_BITS = OFF_MASK + NST * TK * 4;       // NST x 4 words
     static constexpr int OFF_TAKEN = OFF_BITS + NST * 16;          // 16 bytes: the answer of a take-over
     static constexpr int kIds = 2;                                 // items on their way to the other roles
-    static constexpr int OFF_ITEMS = OFF_TAKEN + 16;               // kIds x 32 bytes
-    static constexpr int OFF_BAR = OFF_ITEMS + kIds * 32;
+    static constexpr int OFF_ITEMS = OFF_TAKEN + 16;               // kIds x 48 bytes
+    static constexpr int OFF_BAR = OFF_ITEMS + kIds * 48;
     static constexpr int SMEM = OFF_BAR + 384;
     static constexpr int kReaders = 7;                             // producer, issuer, V rows, four softmax warps
     static constexpr int TMEM_COLS = 256, COL_O = 128, COL_P = 192;
@@ -66,13 +66,15 @@ struct WCfg {
 static_assert(128 * WCfg::REGS_CONTROL + 128 * WCfg::REGS_SOFTMAX <= 65536 / 2, "setmaxnreg moves registers inside the CTA's own share");
 
 struct __align__(16) WItem {
-    int b, head, q0, p0;      // p0: position of the item's first query
+    int b, head, q0;
+    int lo, hi;               // the window of the item's first query
     int a_end, b_lo, b_hi;    // the runs
     int there;                // 0: no further item; 1 + the chunks of the first tokens that share the last tile
     __device__ __forceinline__ int shared() const { return there - 1; }
     __device__ __forceinline__ int tiles_a() const { return there > 1 ? 0 : (a_end + TK - 1) / TK; }
     __device__ __forceinline__ int tiles() const { return tiles_a() + (b_hi - b_lo + TK - 1) / TK; }
 };
+static_assert(sizeof(WItem) == 48, "two of them in WCfg::OFF_ITEMS");
 
 // Asks for the first CTA of the grid that has not started; the answer arrives in shared memory and completes 16 bytes of `bar`.
 __device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
@@ -108,8 +110,10 @@ __device__ __forceinline__ WItem load_item(const TileParams& p, int id) {
     const int rest = id / p.heads;
     it.q0 = (rest % p.n_qb) * TQ;
     it.b = rest / p.n_qb;
-    it.p0 = first_position(p, it.b) + it.q0;
-    const Runs r = visible_runs(p, sequence_keys(p, it.b), it.p0, it.p0 + min(TQ, p.Sq - it.q0) - 1);
+    const Window w = first_window(p, it.b);
+    it.lo = w.lo + it.q0;
+    it.hi = w.hi + it.q0;
+    const Runs r = visible_runs(p, sequence_keys(p, it.b), it.lo, it.hi + min(TQ, p.Sq - it.q0) - 1);
     it.a_end = r.a_end;
     it.b_lo = r.b_lo;
     it.b_hi = r.b_hi;
@@ -436,13 +440,13 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                 continue;
             }
             // what every row of the item sees: keys [all_lo, all_hi] (and the first tokens); what this row does
-            const int all_lo = it.p0 + min(TQ, p.Sq - it.q0) - 1 - p.left, all_hi = it.p0 + p.right;
+            const int all_lo = it.lo + min(TQ, p.Sq - it.q0) - 1, all_hi = it.hi;
             // tiles [0, plain_a) and [plain_lo, plain_hi): every key visible to every row
             const int n_a = it.tiles_a(), plain_a = masked ? 0 : it.a_end / TK;
             const int plain_lo = n_a + (max(all_lo - it.b_lo, 0) + TK - 1) / TK;
             const int plain_hi = masked ? 0 : n_a + max(min(it.b_hi, all_hi + 1) - it.b_lo, 0) / TK;
             int k0 = n_a > 0 ? 0 : it.b_lo, end = n_a > 0 ? it.a_end : it.b_hi;
-            const int row_lo = it.p0 + r_in_tile - p.left, row_hi = it.p0 + r_in_tile + p.right;
+            const int row_lo = it.lo + r_in_tile, row_hi = it.hi + r_in_tile;
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n_tiles; ++j, ++t) {
                 const int own = (min(TK, end - k0) + 31) >> 5, with = j + 1 == n_tiles ? it.shared() : 0, chunks = own + with;
@@ -674,7 +678,7 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     p.k_batch = many ? d->k_batch : d->Sk * d->ldk;
     p.v_batch = many ? d->v_batch : d->Sk * d->ldv;
     p.o_batch = many ? d->o_batch : d->Sq * d->ldo;
-    auto side = [](int64_t w) { return w < 0 || w > kUnlimited ? kUnlimited : static_cast<int>(w); };
+    auto side = [](int64_t w) { return w < 0 || w > kUnlimited ? kUnlimited : static_cast<long long>(w); };
     p.left = side(d->left);
     p.right = side(d->right);
     p.sinks = d->sinks > d->Sk ? p.Sk : static_cast<int>(d->sinks);

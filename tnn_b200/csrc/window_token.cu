@@ -92,8 +92,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
     pdl_wait();   // q, k, v, kv_len and q_start come from earlier kernels; the output may still be read by one
 
     const int rows = min(ROWS, p.Sq * p.group - r0);       // row r = query (r0 + r) / group, head (r0 + r) % group
-    const int p0 = first_position(p, b);
-    const Runs runs = visible_runs(p, sequence_keys(p, b), p0 + r0 / p.group, p0 + (r0 + rows - 1) / p.group);
+    const Window window = first_window(p, b);
+    // keys that every row of the block sees: the window's between these
+    const int all_lo = window.lo + (r0 + rows - 1) / p.group, all_hi = window.hi + r0 / p.group;
+    const Runs runs = visible_runs(p, sequence_keys(p, b), window.lo + r0 / p.group, window.hi + (r0 + rows - 1) / p.group);
     const int n_a = runs.a_end, n = n_a + runs.b_hi - runs.b_lo;
     const int shift = runs.b_lo - n_a;                     // place in the list of visible keys -> key, from place n_a on
     const uint16_t* kp = static_cast<const uint16_t*>(p.k) + b * p.k_batch + kv_head * HD;
@@ -101,8 +103,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
     const float* mask = MASKED ? p.mask_add + static_cast<long long>(b) * p.Sk : nullptr;
     const uint32_t ring_u = smem_u32(ring);
 
-    // keys that every row of the block sees: the window's between these
-    const int all_lo = p0 + (r0 + rows - 1) / p.group - p.left, all_hi = p0 + r0 / p.group + p.right;
     const int tiles = (n + kTile - 1) / kTile;
     const int first = rank * kWarps + warp, step = ctas * kWarps;
     auto fetch = [&](int tile, int stage) {                // tile's keys and values; beyond the last tile an empty group
@@ -134,9 +134,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
             const int r = t * 16 + g + h * 8;
             const bool there = r < rows;
             const int i = there ? (r0 + r) / p.group : 0;
-            const int pos = p0 + i;
-            lo[t][h] = there ? pos - p.left : 1;           // a row that does not exist sees nothing
-            hi[t][h] = there ? pos + p.right : 0;
+            lo[t][h] = there ? window.lo + i : 1;          // a row that does not exist sees nothing
+            hi[t][h] = there ? window.hi + i : 0;
             first_keys[t][h] = there ? p.sinks : 0;
             const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_batch + i * p.ldq + (kv_head * p.group + (there ? (r0 + r) % p.group : 0)) * HD;
 #pragma unroll
@@ -420,7 +419,7 @@ int launch_window_token(const WindowParams& p, int dtype, int sms, cudaStream_t 
     // 37.3 | 25.7 | 31.6 | 32.5; 4 of 4096, 8 heads 21.7 | 14.6 | 10.3 | 7.9.
     const int blocks = (p.Sq * p.group + kBlockRows - 1) / kBlockRows;
     const long long units = static_cast<long long>(p.B) * (p.heads / p.group) * blocks;
-    const long long reach = static_cast<long long>(p.left) + p.right + p.Sq + p.sinks;
+    const long long reach = p.left + p.right + p.Sq + p.sinks;
     const long long keys = p.Sk < reach ? p.Sk : reach;
     int ctas = 1;
     long long least = 0;
