@@ -368,8 +368,12 @@ B200_API int b200_linear_fp8_fwd(const B200LinearFp8Desc* desc, b200_stream_t st
  *   out[b, i, h] = softmax_j(scale * q[b, i, h] . k[b, j, h'] + mask_add[b, j]) . v[b, j, h'],   h' = h / (heads / kv_heads)
  * over the keys j < kv_len[b] with j < sinks or pos - left <= j <= pos + right, where pos = q_start[b] + i is the position
  * of query i.  (The reference has full attention only, as the chain that b200_attention_fwd replaces.)
- *   left, right : window to either side of the query's position; negative = unlimited on that side; right = 0 is causal.
- *   sinks       : how many first keys every query sees (0 = none).
+ *   left, right : window to either side of the query's position; negative = unlimited on that side.
+ *   sinks       : how many first keys every query sees (0 = none), wherever it stands: with causal_sinks = 0 a query at
+ *                 position 0 sees the first token at position 3 too, whatever `right` is.
+ *   causal_sinks: 1 = `right` holds for the first tokens as well, j <= pos + right for every key: they only stay visible to
+ *                 queries whose window has left them behind.  right = 0 with causal_sinks = 1 is causal (with 0 only for
+ *                 sinks <= 1): a text in one call then gives what it gives token by token.  0 or 1.
  *   kv_len      : int32 [B], keys of each sequence (clamped to Sk; <= 0: none), or NULL (= Sk).
  *   q_start     : int32 [B], position of each sequence's first query, or NULL (= 0): Sq new tokens at the end of a cache
  *                 of kv_len keys have q_start = kv_len - Sq.  Any value, beside any left and right: positions are 64-bit.
@@ -399,6 +403,8 @@ typedef struct B200WindowAttentionDesc {
     int32_t        dtype;
     float          scale;
     float          mask_exclude_below;
+    int32_t        causal_sinks;
+    int32_t        reserved_;
 } B200WindowAttentionDesc;
 B200_API int b200_window_attention_fwd(const B200WindowAttentionDesc* desc, b200_stream_t stream);
 

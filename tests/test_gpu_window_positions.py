@@ -80,3 +80,89 @@ def test_positions_and_windows_of_any_size(cuda_device, window, starts, sinks, S
     seen = visible(Sq, 260, window, sinks, [260] * 4, starts, cuda_device)
     check(out, *reference(q, k, v, 4, 2, seen))
     assert bool((out[~seen.any(-1)] == 0).all())
+
+
+# ---------------------------------------------------------------------------------------------------- first tokens, read left to right
+def causal(seen, q_start, right, dev):
+    """`seen` without the keys beyond each query's position + right."""
+    Sq, Sk = seen.shape[1:]
+    pos = torch.arange(Sq, device=dev)[None, :, None] + torch.tensor(q_start, device=dev)[:, None, None]
+    return seen & (torch.arange(Sk, device=dev) <= pos + right)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("left", [0, 20, 100, -1])
+@pytest.mark.parametrize("sinks", [1, 4, 64])
+def test_a_text_in_one_call_is_the_text_token_by_token(cuda_device, sinks, left, dtype):
+    """One call over 200 tokens, pieces of them against the cache so far, and single tokens: every row sees the same keys, so each
+    is within its bound of the one exact result."""
+    n, heads, kv_heads = 200, 4, 2
+    q = _randn(cuda_device, sinks, 1, n, heads * 64).to(dtype)
+    k, v = (_randn(cuda_device, sinks + i, 1, n, kv_heads * 64).to(dtype) for i in (1, 2))
+    seen = causal(visible(n, n, (left, 0), sinks, [n], [0], cuda_device), [0], 0, cuda_device)
+    want, bound = reference(q, k, v, heads, kv_heads, seen)
+    kw = {"window": (left, 0), "sinks": sinks, "causal_sinks": True}
+    check(ops.window_attention(q, k, v, heads, kv_heads, **kw), want, bound)
+    for step in (1, 7, 70):                                  # single tokens and seven in the form for a few, 70 in tiles
+        for at in range(0, n, step):
+            end = min(n, at + step)
+            length = torch.tensor([end], dtype=torch.int32, device=cuda_device)
+            start = torch.tensor([at], dtype=torch.int32, device=cuda_device)
+            k2, v2 = k.clone(), v.clone()
+            k2[:, end:], v2[:, end:] = math.nan, math.nan    # not there yet
+            out = ops.window_attention(q[:, at:end], k2, v2, heads, kv_heads, kv_len=length, q_start=start, **kw)
+            check(out, want[:, at:end], bound[:, at:end])
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Sq", [1, 6, 60, 300])
+@pytest.mark.parametrize("window,sinks,starts", [
+    ((5, 0), 64, [0, 30, 63, 64, 200]), ((40, 3), 50, [0, 44, 49, 52, 300]), ((-1, 0), 200, [0, 100, 199, 250, -20]), ((3, 0), 97, [90, 96, 97, 101, 500]),
+    ((0, 0), 300, [-400, -2, 0, 299, 10 ** 6]), ((10, -1), 20, [0, 5, 600, -100, 19]), ((2 ** 27, 2 ** 26), 9, [-2 ** 26, -2 ** 26 + 4, 2 ** 26, 0, -2 ** 27])])
+def test_causal_first_tokens_at_their_edges(cuda_device, window, sinks, starts, Sq, masked):
+    Sk, lens = 600, [600, 599, 600, 70, 600]
+    q = _randn(cuda_device, Sq, 5, Sq, 256).to(F16)
+    k, v = (_randn(cuda_device, Sq + i, 5, Sk, 128).to(F16) for i in (1, 2))
+    seen = visible(Sq, Sk, window, sinks, lens, starts, cuda_device)
+    if window[1] >= 0:
+        seen = causal(seen, starts, window[1], cuda_device)
+    mask = None
+    if masked:
+        mask = torch.zeros(5, Sk, device=cuda_device)
+        mask[:, 3::5] = -10000.0
+        seen = seen & (mask > -5000)[:, None]
+    out = ops.window_attention(q, k, v, 4, 2, window=window, sinks=sinks, mask_add=mask, causal_sinks=True,
+                               kv_len=torch.tensor(lens, dtype=torch.int32, device=cuda_device),
+                               q_start=torch.tensor(starts, dtype=torch.int32, device=cuda_device))
+    check(out, *reference(q, k, v, 4, 2, seen))
+    assert bool((out[~seen.any(-1)] == 0).all())
+
+
+@pytest.mark.parametrize("Sq", [1, 200])
+def test_keys_of_later_tokens_leave_the_first_row_alone(cuda_device, Sq):
+    q, k, v = (_randn(cuda_device, i, 1, 200, 128).to(F16) for i in range(3))
+    kw = {"window": (64, 0), "sinks": 4, "causal_sinks": True}
+    first = ops.window_attention(q[:, :Sq], k, v, 2, **kw)[0, 0]
+    k[:, 1:] = math.nan
+    if Sq == 1:
+        v[:, 1:] = math.nan                                  # (values that another query of the call sees have to be finite)
+    else:
+        v[:, 1:] = 60000.0
+    assert torch.equal(ops.window_attention(q[:, :Sq], k, v, 2, **kw)[0, 0], first)
+    want, bound = reference(q[:, :1], k[:, :1], v[:, :1], 2, 2, torch.ones(1, 1, 1, dtype=torch.bool, device=cuda_device))
+    check(first[None, None], want, bound)
+
+
+def test_encoder_with_causal_first_tokens(cuda_device):
+    """A stack over a text and over a prefix of it agree on the prefix, bit for bit in tiles that do not depend on the length."""
+    from tnn_b200.encoder import Encoder
+    from tnn_b200.model_synth import EncoderConfig, make_workload
+    wl = make_workload(EncoderConfig(2, 256, 4, 512), 1, 300, seed=3, length_range=(300, 300), num_layers=2)
+    x = torch.from_numpy(wl.x).to(cuda_device)
+    for fp8 in (True, False):
+        enc = Encoder.from_workload(wl, F16, cuda_device, fp8=fp8, window=(40, 0), sinks=4, causal_sinks=True)
+        whole = enc.forward(x)
+        later = x.clone()
+        later[:, 2:] += 1.0                                  # a change behind the first two tokens
+        assert torch.equal(enc.forward(later)[:, :2], whole[:, :2])
+        assert not torch.equal(enc.forward(later)[:, 2:4], whole[:, 2:4])

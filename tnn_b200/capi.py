@@ -93,7 +93,7 @@ class WindowAttentionDesc(_c.Structure):
                 ("q_batch", _i64), ("k_batch", _i64), ("v_batch", _i64), ("o_batch", _i64),
                 ("left", _i64), ("right", _i64), ("sinks", _i64),
                 ("heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32),
-                ("scale", _f32), ("mask_exclude_below", _f32)]
+                ("scale", _f32), ("mask_exclude_below", _f32), ("causal_sinks", _i32), ("reserved_", _i32)]
 
 
 class EncoderLayerWeights(_c.Structure):

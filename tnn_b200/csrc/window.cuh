@@ -26,6 +26,7 @@ struct WindowParams {
     long long ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch;
     long long left, right;              // >= 0, kUnlimited where there is no limit
     int sinks;
+    int causal_sinks;                   // first tokens too are hidden from queries whose window ends before them
     float scale_log2, mask_below;
     int B;
     unsigned int* status;
@@ -49,6 +50,9 @@ __device__ __forceinline__ Window first_window(const WindowParams& p, int b) {
     return w;
 }
 
+// How many first tokens a query sees whose window ends at `hi`.
+__device__ __forceinline__ int first_tokens(const WindowParams& p, int hi) { return p.causal_sinks ? min(p.sinks, hi + 1) : p.sinks; }
+
 // The keys that a run of queries of a sequence can see, as runs [0, a_end) and [b_lo, b_hi); `lo` is where the first one's window
 // begins, `hi` where the last one's ends.
 struct Runs {
@@ -57,6 +61,7 @@ struct Runs {
 __device__ __forceinline__ Runs visible_runs(const WindowParams& p, int kv, int lo, int hi) {
     Runs r;
     r.a_end = min(p.sinks, kv);
+    if (p.causal_sinks) r.a_end = max(0, min(r.a_end, hi + 1));
     r.b_lo = max(0, lo);
     r.b_hi = min(kv, hi + 1);
     if (r.b_hi <= r.b_lo) {                  // nothing but the first tokens

@@ -1,5 +1,7 @@
 // Sliding-window attention with first tokens that stay visible, head_dim 64, grouped key / value heads:
-//   out_i = sum_j p_ij v_j,  p_i = softmax over { j < kv_len : j < sinks or pos_i - left <= j <= pos_i + right } of scale q_i.k_j + mask_j.
+//   out_i = sum_j p_ij v_j,  p_i = softmax over { j < kv_len : j < sinks or pos_i - left <= j <= pos_i + right } of scale q_i.k_j + mask_j
+// (with causal_sinks of the first tokens, too, only j <= pos_i + right; that matters only where the first tokens and the window touch:
+// behind a gap every query of an item is past them).
 //
 // The keys that a block of 128 queries can see are at most two runs: the first tokens [0, sinks) and the window
 // [p_first - left, p_last + right], one run where they touch.  An item (128 queries of one head of one sequence) walks the
@@ -446,7 +448,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             const int plain_lo = n_a + (max(all_lo - it.b_lo, 0) + TK - 1) / TK;
             const int plain_hi = masked ? 0 : n_a + max(min(it.b_hi, all_hi + 1) - it.b_lo, 0) / TK;
             int k0 = n_a > 0 ? 0 : it.b_lo, end = n_a > 0 ? it.a_end : it.b_hi;
-            const int row_lo = it.lo + r_in_tile, row_hi = it.hi + r_in_tile;
+            const int row_lo = it.lo + r_in_tile, row_hi = it.hi + r_in_tile, row_first = first_tokens(p, row_hi);
             float m_run = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n_tiles; ++j, ++t) {
                 const int own = (min(TK, end - k0) + 31) >> 5, with = j + 1 == n_tiles ? it.shared() : 0, chunks = own + with;
@@ -470,7 +472,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t s[32];
-                        uint32_t bits = (low_bits(row_hi + 1 - first) & ~low_bits(row_lo - first)) | low_bits(p.sinks - first);
+                        uint32_t bits = (low_bits(row_hi + 1 - first) & ~low_bits(row_lo - first)) | low_bits(row_first - first);
                         bits &= low_bits(limit - first);
                         first += 32;
                         if (c + 1 == own) {
@@ -636,7 +638,8 @@ bool set_window_attributes(int dev) {
 extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_stream_t stream_) {
     using namespace b200;
     if (!d || !d->q || !d->k || !d->v || !d->out) return B200_ERR_PARAM;
-    if (d->B < 0 || d->Sq < 0 || d->Sk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads || d->sinks < 0)
+    if (d->B < 0 || d->Sq < 0 || d->Sk <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->heads % d->kv_heads || d->sinks < 0 ||
+        (d->causal_sinks != 0 && d->causal_sinks != 1))
         return B200_ERR_PARAM;
     if (d->head_dim != HD) return B200_ERR_UNSUPPORTED;
     if (!is_half_dtype(d->dtype)) return B200_ERR_PARAM;
@@ -682,6 +685,7 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     p.left = side(d->left);
     p.right = side(d->right);
     p.sinks = d->sinks > d->Sk ? p.Sk : static_cast<int>(d->sinks);
+    p.causal_sinks = d->causal_sinks;
     p.scale_log2 = d->scale * kLog2e;
     p.mask_below = d->mask_exclude_below > kLeastMask ? d->mask_exclude_below : kLeastMask;
     p.status = device_status_ptr();

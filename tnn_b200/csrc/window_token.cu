@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
             const int i = there ? (r0 + r) / p.group : 0;
             lo[t][h] = there ? window.lo + i : 1;          // a row that does not exist sees nothing
             hi[t][h] = there ? window.hi + i : 0;
-            first_keys[t][h] = there ? p.sinks : 0;
+            first_keys[t][h] = there ? first_tokens(p, hi[t][h]) : 0;
             const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_batch + i * p.ldq + (kv_head * p.group + (there ? (r0 + r) % p.group : 0)) * HD;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {

@@ -26,9 +26,11 @@ class Encoder:
         self.fp8 = False          # matrix weights in block-scaled e4m3
         self.window = None        # (left, right): sliding-window attention
         self.sinks = 0
+        self.causal_sinks = False
 
     @classmethod
-    def from_workload(cls, wl, dtype=torch.float16, device="cuda", fold_layernorm=False, fp8=False, window=None, sinks=0):
+    def from_workload(cls, wl, dtype=torch.float16, device="cuda", fold_layernorm=False, fp8=False, window=None, sinks=0,
+                      causal_sinks=False):
         """`fold_layernorm`: prepare the weights for the five-launch form of a layer (both LayerNorms folded into
         the neighbouring GEMMs); only full encoder layers can be folded.  Off by default: at BERT's K = 768 the
         seven-launch layer with its own LayerNorm kernel is the faster one, and it is what the TNN plug-in runs.
@@ -36,10 +38,11 @@ class Encoder:
         For long documents: `fp8` keeps the matrix weights in e4m3 with a scale per 128 x 128 block and runs the four GEMMs
         of a layer on 8-bit operands (activations between launches stay in `dtype`, the feed-forward's inner one in 8 bits);
         `window=(left, right)` lets every token see that many neighbours and the first `sinks` tokens only.  A sequence whose
-        keys are all masked then yields an attention output of zeros."""
+        keys are all masked then yields an attention output of zeros.  `causal_sinks` (for `right` = 0): a token sees no first
+        token behind itself."""
         enc = cls(wl.cfg, dtype, torch.device(device))
         enc.fold = bool(fold_layernorm) and wl.cfg.with_ffn
-        enc.fp8, enc.window, enc.sinks = bool(fp8), window, int(sinks)
+        enc.fp8, enc.window, enc.sinks, enc.causal_sinks = bool(fp8), window, int(sinks), bool(causal_sinks)
         if enc.fold and (enc.fp8 or window is not None):
             raise ValueError("fold_layernorm is a form of the half-precision, full-attention layer")
         H, F = wl.cfg.hidden, wl.cfg.ffn
@@ -100,7 +103,7 @@ class Encoder:
             return ops.attention(qkv, cfg.heads, m2, kv_len, scale=scale)
         H = cfg.hidden
         return ops.window_attention(qkv[..., :H], qkv[..., H:2 * H], qkv[..., 2 * H:], cfg.heads, window=self.window,
-                                    sinks=self.sinks, mask_add=m2, kv_len=kv_len, scale=scale)
+                                    sinks=self.sinks, mask_add=m2, kv_len=kv_len, scale=scale, causal_sinks=self.causal_sinks)
 
     def _fp8_stack(self, h, m2, kv_len, out=None):
         """The layers on 8-bit operands: h `[B,S,H]` half precision -> the same; nine launches a layer and a quantizer in

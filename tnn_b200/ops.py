@@ -480,10 +480,11 @@ def _per_sequence(t, B, what):
 
 
 def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, mask_add=None, kv_len=None, q_start=None,
-                     scale=None, exclude_below=-5000.0, out=None):
+                     scale=None, exclude_below=-5000.0, out=None, causal_sinks=False):
     """Attention of q `[B, Sq, heads*64]` over k, v `[B, Sk, kv_heads*64]` (views of a packed QKV activation will do) ->
     `[B, Sq, heads*64]`.  A query at position p sees the keys j < kv_len with j < sinks or p - left <= j <= p + right,
-    `window` = (left, right), negative = unlimited on that side.
+    `window` = (left, right), negative = unlimited on that side.  `causal_sinks`: j <= p + right for the first keys too; a text
+    read left to right (right = 0) with more than one of them needs it, or its first queries see tokens behind themselves.
 
     kv_len `[B]` int32: keys of each sequence (None: all Sk).  q_start `[B]` int32: position of each sequence's first query
     (None: 0); Sq new tokens at the end of a cache have q_start = kv_len - Sq.  mask_add fp32 `[B, Sk]`: additive key mask, a
@@ -521,7 +522,7 @@ def window_attention(q, k, v, heads, kv_heads=None, window=(-1, -1), sinks=0, ma
     d = capi.WindowAttentionDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), capi.ptr(mask_add), capi.ptr(kv_len), capi.ptr(q_start),
                                  out.data_ptr(), B, Sq, Sk, ldq, ldk, ldv, ldo, q_batch, k_batch, v_batch, o_batch, window[0],
                                  window[1], sinks, heads, kv_heads, 64, capi.dtype_code(dtype), 0.125 if scale is None else scale,
-                                 exclude_below)
+                                 exclude_below, 1 if causal_sinks else 0)
     if B and Sq:
         _call("b200_window_attention_fwd", d, index)
     return out
