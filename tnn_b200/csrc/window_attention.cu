@@ -84,7 +84,8 @@ __device__ __forceinline__ void take_over(void* answer, uint64_t* bar) {
                  ::"r"(smem_u32(answer)), "r"(smem_u32(bar))
                  : "memory");
 }
-// Its block index, or -1 if every CTA has started.
+// Its block index, or -1 if every CTA has started.  The slot is read through the generic proxy and written by the next request
+// through the async one: the fence keeps that write behind this read (an item would be lost or done twice).
 __device__ __forceinline__ int taken_over(const void* answer) {
     uint32_t ok, x;
     asm volatile(
@@ -97,6 +98,7 @@ __device__ __forceinline__ int taken_over(const void* answer) {
         : "=r"(ok), "=r"(x)
         : "r"(smem_u32(answer))
         : "memory");
+    fence_async_proxy_shared();
     return ok ? static_cast<int>(x) : -1;
 }
 struct WTile {
