@@ -145,9 +145,6 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                         if (++st == STAGES) { st = 0; ph ^= 1u; }
                     }
                 }
-                if (!ok) {
-                    for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
-                }
             }
         } else if (warp == 1) {
             // -------------------------------------------------------- UMMA issuer
@@ -464,6 +461,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {
+        if (*abort_flag != 0) let_copies_land();
         tcgen05_fence_after();
         tmem_dealloc(tmem_base, C::TMEM_COLS);
     }

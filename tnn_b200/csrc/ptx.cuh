@@ -328,6 +328,11 @@ __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.
 
 __device__ __forceinline__ void nanosleep(uint32_t ns) { asm volatile("nanosleep.u32 %0;" ::"r"(ns)); }
 
+// The end of a CTA that gave a wait up: whatever any of its roles has still in flight (TMA loads, UMMAs and their commits, the answer
+// of a take-over) gets 640 us to arrive, before the shared memory and TMEM that it writes go to the next CTA.
+__device__ __forceinline__ void let_copies_land() {
+    for (int i = 0; i < 64; ++i) nanosleep(10000);
+}
 
 // ---------------------------------------------------------------- programmatic dependent launch
 // A kernel launched with the programmatic-stream-serialization attribute may start while its predecessor in the stream

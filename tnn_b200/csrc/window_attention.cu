@@ -284,9 +284,6 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                     }
                 }
             }
-            if (!ok && lane == 0) {
-                for (int i = 0; i < 64; ++i) nanosleep(10000);   // let copies in flight land
-            }
             __syncwarp();
         } else if (warp == 1) {
             // ------------------------------------------------------------ UMMA issuer
@@ -615,6 +612,7 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {
+        if (*abort_flag != 0) let_copies_land();
         tcgen05_fence_after();
         tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
