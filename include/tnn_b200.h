@@ -383,8 +383,9 @@ B200_API int b200_linear_fp8_fwd(const B200LinearFp8Desc* desc, b200_stream_t st
  *   window, at or beyond kv_len, or dropped by mask_add) may hold anything, infinities and NaN included; a row that some
  *   query sees has to be finite for the others' results.
  *   q [B, Sq, ldq], k, v [B, Sk, ld*], out [B, Sq, ldo] : dtype (F16 / BF16), head h at columns h * 64; *_batch = elements
- *   from one sequence to the next.  Requirements: head_dim == 64, kv_heads divides heads, all strides % 8 == 0, 16-byte
- *   aligned pointers, Sq, Sk <= 2^24.
+ *   from one sequence to the next (larger or smaller than ld*: sequences behind one another, or [S, B, ld*]).  Rows of out do
+ *   not overlap.  Requirements: head_dim == 64, kv_heads divides heads, all strides % 8 == 0, 16-byte aligned pointers,
+ *   Sq <= 2^24, 1 <= Sk <= 2^24.  A mask_add value of 2^127 or more gives NaN.
  */
 typedef struct B200WindowAttentionDesc {
     const void*    q;

@@ -166,3 +166,29 @@ def test_encoder_with_causal_first_tokens(cuda_device):
         later[:, 2:] += 1.0                                  # a change behind the first two tokens
         assert torch.equal(enc.forward(later)[:, :2], whole[:, :2])
         assert not torch.equal(enc.forward(later)[:, 2:4], whole[:, 2:4])
+
+
+# ---------------------------------------------------------------------------------------------------- layouts
+@pytest.mark.parametrize("B,Sq,Sk", [(3, 150, 150), (3, 1, 400), (5, 40, 333), (2, 6, 90)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_sequences_side_by_side(cuda_device, B, Sq, Sk, dtype):
+    """`[S, B, width]` tensors, seen as `[B, S, width]`: the stride from one sequence to the next is the smaller one."""
+    q = _randn(cuda_device, 1, Sq, B, 256).to(dtype)
+    k, v = (_randn(cuda_device, i, Sk, B, 128).to(dtype) for i in (2, 3))
+    starts, lens = [Sk - Sq - b for b in range(B)], [Sk - b for b in range(B)]
+    kw = {"window": (64, 3), "sinks": 2, "q_start": torch.tensor(starts, dtype=torch.int32, device=cuda_device),
+          "kv_len": torch.tensor(lens, dtype=torch.int32, device=cuda_device)}
+    back = torch.full((Sq + 2, B, 272), 7.0, dtype=dtype, device=cuda_device)
+    views = [t.transpose(0, 1) for t in (q, k, v)]
+    got = ops.window_attention(*views, 4, 2, out=back[1:Sq + 1, :, :256].transpose(0, 1), **kw)
+    check(got, *reference(*views, 4, 2, visible(Sq, Sk, (64, 3), 2, lens, starts, cuda_device)))
+    assert torch.equal(got, ops.window_attention(*(t.contiguous() for t in views), 4, 2, **kw))
+    assert bool((back[0] == 7).all()) and bool((back[-1] == 7).all()) and bool((back[..., 256:] == 7).all())
+
+
+def test_an_output_whose_rows_overlap_is_refused(cuda_device):
+    q = torch.zeros(2, 5, 128, dtype=F16, device=cuda_device)
+    for strides in ((256, 128, 1), (64, 128, 1), (512, 128, 1), (128, 248, 1), (120, 256, 1)):
+        out = torch.empty(5000, dtype=F16, device=cuda_device).as_strided((2, 5, 128), strides)
+        with pytest.raises(capi.B200Error):
+            ops.window_attention(q, q, q, 2, out=out)

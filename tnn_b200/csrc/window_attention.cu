@@ -647,7 +647,10 @@ extern "C" int b200_window_attention_fwd(const B200WindowAttentionDesc* d, b200_
     if ((d->ldq % 8) || (d->ldk % 8) || (d->ldv % 8) || (d->ldo % 8)) return B200_ERR_PARAM;
     if ((d->q_batch % 8) || (d->k_batch % 8) || (d->v_batch % 8) || (d->o_batch % 8)) return B200_ERR_PARAM;
     if (d->ldq < wq || d->ldk < wk || d->ldv < wk || d->ldo < wq) return B200_ERR_PARAM;
-    if (d->B > 1 && (d->q_batch <= 0 || d->k_batch <= 0 || d->v_batch <= 0 || d->o_batch < (d->Sq - 1) * d->ldo + wq))
+    if (d->B > 1 && (d->q_batch <= 0 || d->k_batch <= 0 || d->v_batch <= 0)) return B200_ERR_PARAM;
+    // no row of the output in two places: sequences behind one another, or their rows interleaved ([Sq, B, width])
+    if (d->B > 1 && d->Sq > 0 && !(d->o_batch >= wq && (d->o_batch - wq) / d->ldo >= d->Sq - 1) &&
+        !(d->o_batch >= wq && (d->ldo - wq) / d->o_batch >= d->B - 1))
         return B200_ERR_PARAM;
     if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out)) return B200_ERR_PARAM;
     if (d->mask_add && d->mask_exclude_below != d->mask_exclude_below) return B200_ERR_PARAM;
