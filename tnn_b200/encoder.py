@@ -226,6 +226,8 @@ class Encoder:
         windows: through the operators)."""
         if not self.cfg.with_ffn:
             raise ValueError("b200_encoder_fwd runs full encoder layers; use forward_ops for attention-only blocks")
+        if hidden.dtype != self.dtype or not hidden.is_contiguous():   # it is written through its address, row behind row
+            raise ValueError("hidden: contiguous %s" % self.dtype)
         if self.fp8 or self.window is not None:   # launch by launch; the last LayerNorm writes the result in place
             (self._fp8_stack if self.fp8 else self._half_stack)(hidden, mask2d, kv_len, out=hidden)
             return hidden
