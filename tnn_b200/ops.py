@@ -18,15 +18,16 @@ def _require_cuda(*ts):
             raise ValueError("tnn_b200 operators take CUDA tensors only (there is no CPU path)")
 
 
-def _rows(t, width, at_least=0):
+def _rows(t, width, at_least=0, written=False):
     """`t` as rows of `width` elements: (tensor that holds them, number of rows, row stride).  A contiguous tensor, the
     usual one, needs no view of its own: making views costs more than filling a descriptor.  What does not divide into
-    such rows is refused by `reshape`; so are fewer than `at_least` rows, which a kernel would reach beyond."""
+    such rows is refused by `reshape`; so are fewer than `at_least` rows, which a kernel would reach beyond, and, where the
+    kernel writes, what could only be copied: the results would be lost with the copy."""
     if t.is_contiguous() and width and t.numel() % width == 0:
         rows, ld = t.numel() // width, width
     else:
-        t = t.reshape(-1, width)
-        assert t.stride(1) == 1
+        given, t = t, t.reshape(-1, width)
+        assert t.stride(1) == 1 and not (written and t.data_ptr() != given.data_ptr()), "out: rows that need no copy"
         rows, ld = t.shape[0], t.stride(0)
     assert rows >= at_least, "fewer rows than the input has"
     return t, rows, ld
@@ -88,7 +89,7 @@ def _linear_desc(x, w_nk, bias, residual, epilogue, out_dtype, out, block_n, out
     x2, M, ldx = _rows(x, K)
     if out is None:
         out = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype or x.dtype, device=x.device)
-    y2, _, ldy = _rows(out, N, M)
+    y2, _, ldy = _rows(out, N, M, True)
     d = capi.LinearDesc(x2.data_ptr(), w_nk.data_ptr(), capi.ptr(bias), None, y2.data_ptr(), M, N, K, ldx,
                         w_nk.stride(0), 0, ldy, capi.dtype_code(x.dtype), capi.dtype_code(out.dtype), epilogue, block_n)
     if residual is not None:
@@ -161,7 +162,7 @@ def _layernorm_desc(x, gamma, beta, eps, residual, out_dtype, out):
     x2, rows, ldx = _rows(x, H)
     if out is None:
         out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-    y2, _, ldy = _rows(out, H, rows)
+    y2, _, ldy = _rows(out, H, rows, True)
     d = capi.LayerNormDesc(x2.data_ptr(), None, gamma.data_ptr(), beta.data_ptr(), y2.data_ptr(), rows, H, ldx, 0, ldy,
                            capi.dtype_code(x.dtype), capi.dtype_code(out.dtype), float(eps))
     if residual is not None:
