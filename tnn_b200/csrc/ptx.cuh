@@ -221,7 +221,7 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
                  : "memory");
 }
 
-// The commit of kernels whose UMMAs are umma_f8_*.
+// umma_commit under the name that goes with umma_f8_ss: the source tests find each kind of commit beside its own UMMAs.
 __device__ __forceinline__ void umma_f8_commit(uint64_t* bar) { umma_commit(bar); }
 
 // TMEM -> registers: lane (base lane + threadIdx%32), 32 consecutive 32-bit columns starting at taddr's column.
