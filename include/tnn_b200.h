@@ -339,7 +339,8 @@ B200_API int b200_add_layernorm_fp8_fwd(const B200LayerNormFp8Desc* desc, b200_s
  * in an order fixed by the shapes and out_dtype): a row's result depends on no other row, and above 128 rows not on M.
  *   x [M, K], w_nk [N, K]: e4m3;  bias: fp32 [N] or NULL;  residual: res_dtype (F16 or BF16)
  *   y: out_dtype F16, BF16, F32, or E4M3 with y_scale[ceil(N / 128), ld_y_scale] (the operand of a following 8-bit GEMM).
- *   GELU is within 4e-6 of the erf form, tanh the hardware's (relative error 2^-11) unless y is F32 (both then to fp32).
+ *   GELU is within 4e-6 of the erf form, tanh within a relative 2^-11 (calls of up to 128 rows may get it to fp32) unless y is
+ *   F32 (both then to fp32).
  *   Requirements: K % 16 == 0, N % 8 == 0 (16 for E4M3), ldx, ldw % 16 == 0, ldy % 8 == 0 (16), ldr % 8 == 0, K <= 2^24,
  *   ld_x_scale and ld_y_scale >= M, 16-byte aligned pointers (scales: 4-byte).
  *   block_n: 0 = choose the tile; 64 (not for E4M3), 128, 256: tiles of 128 x block_n; -1: the form

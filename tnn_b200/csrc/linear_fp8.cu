@@ -6,7 +6,8 @@
 // fresh accumulator in a TMEM buffer, and the epilogue warps add scale * buffer to fp32 sums that stay in their registers for
 // the whole tile (thread = row, COLS columns), while the tensor pipe fills the other buffers.  Products are exact in fp32; the
 // sum inside a block is the tensor core's fp32 accumulation, the sum over blocks one fp32 FMA each, in ascending order whatever
-// the tile, so a row's result depends on neither the batch nor the tile chosen.
+// the tile, so among the tiles of this file a row's result depends on neither the batch nor the tile chosen (calls of up to 128
+// rows may go to linear_fp8_rows.cu, which adds in another order).
 //
 // A tile is 128 x BN on one SM.
 //   warp 0      : TMA producer
@@ -16,8 +17,12 @@
 //
 // What bounds it is the chain of a TMEM buffer: UMMAs, commit, reads, hand-back; the reads and the next k-block's accumulation
 // share TMEM.  On 256 columns a k-block costs 0.48 us (its UMMAs alone 0.32), a tile 2.6 us beside its k-blocks.
-// 16384 x 4096 x 4096 with an f16 result 293 us (1870 TFLOP/s), K = 1024 101 us, f32 110, e4m3 102 (with GELU 128), GELU 123, residual 133.
-// Pairs of CTAs on 256 x 256 and 256 x 128 tiles took 107 and 113 us at K = 1024, two CTAs per SM on 128 x 128 95 but 157 with GELU.
+// 16384 x 4096 x 4096 with an f16 result 277 to 300 us (1830 to 1980 TFLOP/s; 14 waves at those costs would take 252, but at K = 4096
+// the clock gives way to the power limit), K = 1024 96 to 107 us, f32 108, e4m3 with GELU 121, 4096 -> 1024 with a residual 92.
+// Pairs of CTAs on 256 x 256 and 256 x 128 tiles took 107 and 113 us at K = 1024.  Two CTAs per SM on 128 x 128 tiles, against this form
+// then: bias 95 | 95, f32 106 | 111, e4m3 94 | 102, but GELU 157 | 128 and residual 160 | 124.
+// ops.linear on half-precision operands is the faster one from 128 rows on at K = 768 and 1024 (16384 rows 1024 -> 4096 93 | 107 us); this
+// one is for half the weight bytes, for a few rows (1.2 to 3 times) and for K of some thousands (16384 x 4096 x 4096 357 | 300).
 // For up to 128 rows and few columns linear_fp8_rows.cu does the same without a pipeline.
 #include "fp8.cuh"
 #include "linear_common.cuh"
@@ -333,6 +338,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                 } else if (p.epilogue == B200_EPI_BIAS_TANH) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
+                        // (2^-11 relative: an error of the size of an f16 result's own rounding, less than bf16's and e4m3's; one
+                        // instruction, where tanhf is some twenty.  linear_fp8_rows.cu has the time for tanhf.)
                         if (OUT == kOutF32) v[j] = tanhf(v[j]);
                         else asm("tanh.approx.f32 %0, %1;" : "=f"(v[j]) : "f"(v[j]));
                     }
@@ -561,7 +568,9 @@ int validate_linear_fp8(const B200LinearFp8Desc* d) {
 }
 
 // The tile of the smallest estimated time: waves of tiles over the SMs x (per tile + per k-block) + what the last tile's epilogue
-// adds, in us, fitted to launches measured in a CUDA graph; over 60 drawn shapes the choice costs 0.2 % more than the best.
+// adds, in us, fitted to launches measured in a CUDA graph; over 60 drawn shapes the choice costs 0.2 % more than the best, over 42
+// of six widths (K = 1024 to 4096) and 200 to 16384 rows 2.8 % at most.  (Many waves at K = 4096 take 10 to 19 % longer than estimated,
+// on every width: the clock falls.)
 // us per launch on 64 | 128 | 256 columns:  777 rows 768 -> 2304 7.5 | 6.0 | 8.0, 1024 -> 1024 5.6 | 6.4 | 8.8, 1024 -> 4096
 // 13.7 | 10.5 | 9.5;  1300 rows 1024 -> 1024 8.2 | 6.6 | 8.9, 4096 -> 1024 22.1 | 15.2 | 21.2;  4096 rows 1024 -> 1024
 // 14.4 | 10.8 | 9.4;  8192 rows 1024 -> 4096 81 | 57 | 49;  41339 rows 480 -> 832 59.8 | 39.9 | 45.2.

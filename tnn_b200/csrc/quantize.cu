@@ -9,7 +9,7 @@ namespace {
 // ---------------------------------------------------------------- rows -> e4m3 + scales
 // A group of 8 lanes owns one block of 128 values, 16 per lane: 16-byte loads and one 16-byte store per lane, the block's
 // largest magnitude by three shuffles.  A warp holds four blocks, UNROLL of them per lane in flight.  65536 x 1024 bf16: 34.5 us,
-// 0.90 of the measured copy rate.
+// 0.90 of the measured copy rate; f32 56.9 us, 0.91.
 template <int DT>
 struct Raw16 {   // 16 consecutive elements as loaded
     static constexpr int Q = DT == B200_F32 ? 4 : 2;

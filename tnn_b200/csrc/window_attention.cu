@@ -14,8 +14,9 @@
 // are not dealt in advance: the grid has a CTA per item, and a running CTA takes over the next one that has not started
 // (cluster launch control), prefetching its queries and scores while it is still at work on its own.
 //
-// 16384 causal queries, window 1024, 4 sinks, 16 / 4 heads, bf16: 142 us (67 GFLOP visible; the exp unit's floor is 58), 4 x 4096 queries,
-// window 256 to both sides, ragged: 59 to 67 us.  First tokens that share a tile: 11 x 1302 queries, window 142 to both sides, 16 sinks
+// 16384 causal queries, window 1024, 4 sinks, 16 / 4 heads, bf16: 141 us (67 GFLOP visible; the exp unit's floor is 58), 4 x 4096 queries,
+// window 256 to both sides, ragged: 59 to 67 us.  With an additive mask, where every tile takes the edges' path, 190 and 77 (padding
+// belongs in kv_len).  First tokens that share a tile: 11 x 1302 queries, window 142 to both sides, 16 sinks
 // 69 -> 64 us, 16 x 393, window 6, 28 -> 24.7; windows of whole tiles pay up to 2 % for it (139.6 -> 142).  The exp unit is 56 % busy: the two softmax warps of a scheduler wait for fixed
 // latencies and tend to be in the exp pass together.  Exponentials by a polynomial (1/4 of them 153 us), two threads per row
 // (140), both passes rolled (155) did not help.
@@ -537,6 +538,9 @@ window_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (c < chunks) {
+                        // The weights are rounded to the operands' type for PV, half a step of it each (2^-11, 2^-8) and independent
+                        // of one another: 2.3e-3 of the result's norm in bf16 where its own rounding is 1.7e-3.  A second product
+                        // with what the rounding left would double PV and its conversions.  Their sum is kept unrounded.
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {

@@ -1,4 +1,5 @@
-// Window attention of a few query tokens against a long cache (head_dim 64): HBM-bound, every visible key and value once.
+// Window attention of a few query tokens against a long cache (head_dim 64): HBM-bound, every visible key and value once per block of
+// up to 32 query rows (33 to 64 rows of a sequence stream them twice, the second time mostly from L2).
 //
 // The queries of one sequence whose heads share a key / value head (Sq x group rows) are one matrix, in blocks of MT x 16 rows.
 // The visible keys, the first tokens and the window behind one another, are dealt in tiles of 32 to the warps of a cluster of
@@ -21,7 +22,16 @@ constexpr int kStages = 3;
 constexpr int kStageBytes = 2 * kTile * HD * 2;            // K and V
 constexpr int kRingBytes = kStages * kStageBytes;          // one warp's
 constexpr int kBlockRows = 32;                             // query rows per block at most
-constexpr int kMaxRows = 64;                               // beyond, the tile kernel
+// Beyond this many rows (queries x heads of a group) the tile kernel takes over.  us, this kernel | tiles (one query tile of one head per
+// CTA, keys not split), unlimited window, rows x keys:
+//   1 sequence, 12 / 12 heads: 64 x 1024 9.8 | 14.4   72 x 1024 14.6 | 14.3   64 x 32768 52 | 315   128 x 32768 92 | 315   512 x 32768 268 | 354
+//   1 sequence, 12 / 1 heads:  72 x 32768 36 | 314   192 x 32768 37 | 314
+//   8 sequences, 16 / 4 heads: 64 x 8192 29 | 111   192 x 8192 84 | 111   512 x 8192 176 | 112
+//   32 sequences, 16 / 4:      64 x 1024 17 | 36   128 x 1024 32 | 36   192 x 1024 47 | 37   192 x 8192 264 | 230   512 x 32768 2310 | 901
+// So up to 64 rows this kernel is never behind; beyond, either may be, by up to nine times, depending on the number of sequences and
+// the length of the cache.  The limit looks at the rows of a single sequence alone: with more than 64 of them a row's result depends
+// neither on the batch nor on the length of the cache it lies in.
+constexpr int kMaxRows = 64;
 
 template <int MT>
 constexpr int token_smem() { return kWarps * kRingBytes + (2 * kWarps + 2) * MT * 16 * 4; }
@@ -256,6 +266,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) window_token_kernel(const Wind
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {                      // 16 keys each
+            // The weights are rounded to the operands' type for this product, half a step of it each (2^-11, 2^-8) and independent
+            // of one another: 2.2e-3 of the result's norm in bf16 where its own rounding is 1.7e-3.  Their sum is kept unrounded.
             uint32_t pf[MT][4];
 #pragma unroll
             for (int t = 0; t < MT; ++t) {

@@ -36,7 +36,9 @@ class Encoder:
         seven-launch layer with its own LayerNorm kernel is the faster one, and it is what the TNN plug-in runs.
 
         For long documents: `fp8` keeps the matrix weights in e4m3 with a scale per 128 x 128 block and runs the four GEMMs
-        of a layer on 8-bit operands (activations between launches stay in `dtype`, the feed-forward's inner one in 8 bits);
+        of a layer on 8-bit operands (activations between launches stay in `dtype`, the feed-forward's inner one in 8 bits).
+        It halves the bytes of the weights; at hidden sizes of 768 and 1024 a layer takes 1.2 to 1.5 times as long as in half
+        precision.  Padding costs less in `kv_len` than in a mask (`forward_hidden`), where a window is set;
         `window=(left, right)` lets every token see that many neighbours and the first `sinks` tokens only.  A sequence whose
         keys are all masked then yields an attention output of zeros.  `causal_sinks` (for `right` = 0): a token sees no first
         token behind itself."""
@@ -106,7 +108,7 @@ class Encoder:
                                     sinks=self.sinks, mask_add=m2, kv_len=kv_len, scale=scale, causal_sinks=self.causal_sinks)
 
     def _fp8_stack(self, h, m2, kv_len, out=None):
-        """The layers on 8-bit operands: h `[B,S,H]` half precision -> the same; nine launches a layer and a quantizer in
+        """The layers on 8-bit operands: h `[B,S,H]` half precision -> the same; eight launches a layer and a quantizer in
         front of the first.  Every LayerNorm also writes the 8-bit operand of the GEMMs behind it."""
         cfg = self.cfg
         codes, scales = ops.quantize_fp8(h)
