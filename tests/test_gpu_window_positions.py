@@ -115,7 +115,7 @@ def test_a_text_in_one_call_is_the_text_token_by_token(cuda_device, sinks, left,
 
 
 @pytest.mark.parametrize("masked", [False, True])
-@pytest.mark.parametrize("Sq", [1, 6, 60, 300])
+@pytest.mark.parametrize("Sq", [1, 6, 25, 60, 300])   # 2, 12, 50 rows (two blocks) in the form for a few, the others in tiles
 @pytest.mark.parametrize("window,sinks,starts", [
     ((5, 0), 64, [0, 30, 63, 64, 200]), ((40, 3), 50, [0, 44, 49, 52, 300]), ((-1, 0), 200, [0, 100, 199, 250, -20]), ((3, 0), 97, [90, 96, 97, 101, 500]),
     ((0, 0), 300, [-400, -2, 0, 299, 10 ** 6]), ((10, -1), 20, [0, 5, 600, -100, 19]), ((2 ** 27, 2 ** 26), 9, [-2 ** 26, -2 ** 26 + 4, 2 ** 26, 0, -2 ** 27])])
@@ -192,3 +192,32 @@ def test_an_output_whose_rows_overlap_is_refused(cuda_device):
         out = torch.empty(5000, dtype=F16, device=cuda_device).as_strided((2, 5, 128), strides)
         with pytest.raises(capi.B200Error):
             ops.window_attention(q, q, q, 2, out=out)
+
+
+@pytest.mark.parametrize("Sq", [1, 25, 130])
+def test_causal_first_tokens_captured_and_on_two_streams(cuda_device, Sq):
+    k, v = (_randn(cuda_device, i, 2, 500, 128).to(F16) for i in (1, 2))
+    cases = [(_randn(cuda_device, 5 + i, 2, Sq, 256).to(F16), s) for i, s in enumerate(([0, 3], [300, 40], [2 ** 30, -50]))]
+    start = lambda s: torch.tensor(s, dtype=torch.int32, device=cuda_device)   # noqa: E731
+
+    def call(q, s):
+        return ops.window_attention(q, k, v, 4, 2, window=(30, 0), sinks=70, q_start=s, causal_sinks=True)
+
+    want = [call(q, start(s)) for q, s in cases]
+    for (q, s), w in zip(cases, want):
+        seen = causal(visible(Sq, 500, (30, 0), 70, [500, 500], s, cuda_device), s, 0, cuda_device)
+        check(w, *reference(q, k, v, 4, 2, seen))
+    q0, s0 = cases[0][0].clone(), start(cases[0][1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(q0, s0)
+    side = torch.cuda.Stream()
+    for (q, s), w in zip(cases, want):
+        q0.copy_(q)
+        s0.copy_(start(s))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            eager = call(q0, s0)
+        torch.cuda.synchronize()
+        assert torch.equal(out, w) and torch.equal(eager, w)
