@@ -338,8 +338,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
                 } else if (p.epilogue == B200_EPI_BIAS_TANH) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        // (2^-11 relative: an error of the size of an f16 result's own rounding, less than bf16's and e4m3's; one
-                        // instruction, where tanhf is some twenty.  linear_fp8_rows.cu has the time for tanhf.)
+                        // (2^-11 relative: an error of the size of an f16 result's own rounding, less than bf16's and e4m3's; the
+                        // epilogue's instructions are what a tile waits for.  linear_fp8_rows.cu, which waits for memory, calls tanhf.)
                         if (OUT == kOutF32) v[j] = tanhf(v[j]);
                         else asm("tanh.approx.f32 %0, %1;" : "=f"(v[j]) : "f"(v[j]));
                     }

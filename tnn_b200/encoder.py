@@ -38,10 +38,9 @@ class Encoder:
         For long documents: `fp8` keeps the matrix weights in e4m3 with a scale per 128 x 128 block and runs the four GEMMs
         of a layer on 8-bit operands (activations between launches stay in `dtype`, the feed-forward's inner one in 8 bits).
         It halves the bytes of the weights; at hidden sizes of 768 and 1024 a layer takes 1.2 to 1.5 times as long as in half
-        precision.  Padding costs less in `kv_len` than in a mask (`forward_hidden`), where a window is set;
-        `window=(left, right)` lets every token see that many neighbours and the first `sinks` tokens only.  A sequence whose
+        precision.  `window=(left, right)` lets every token see that many neighbours and the first `sinks` tokens only.  A sequence whose
         keys are all masked then yields an attention output of zeros.  `causal_sinks` (for `right` = 0): a token sees no first
-        token behind itself."""
+        token behind itself.  With a window, padding costs less as `kv_len` alone (`forward_hidden`) than as a mask."""
         enc = cls(wl.cfg, dtype, torch.device(device))
         enc.fold = bool(fold_layernorm) and wl.cfg.with_ffn
         enc.fp8, enc.window, enc.sinks, enc.causal_sinks = bool(fp8), window, int(sinks), bool(causal_sinks)
